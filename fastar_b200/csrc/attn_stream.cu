@@ -42,6 +42,7 @@ constexpr int D_V = 512;
 constexpr int CHUNK = TILE * 128;      // 8 KB: [64 tok x 64 dims]
 constexpr int P_BYTES = HEADS * TILE * 2;  // 8 KB
 constexpr int ST_THREADS = 448;  // warps: 0, 10, 11 copy; 1, 13 issue QK; 12 issues SV; 2-9 softmax
+constexpr int E8_THREADS = 512;  // E4M3 cache: 0 copies; 1, 10 issue QK (1: the Q_eff copies too); 11 issues SV; 12-15 dequantise
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t COL_Q = 0, COL_S = 288, COL_O = 0;
 constexpr uint32_t LANE16 = 16u << 16;
@@ -60,13 +61,26 @@ constexpr float RESCALE_THRESHOLD = 8.0f;
 // buffer it had to); it waits for them only in the rare case that it rescales O.  Worth 1.3 us
 // of 85 on the batched-decode workload: the kernel is not bound by that dependency.
 constexpr int MISC_BYTES = 2048;
-__host__ __device__ constexpr int off_pbuf(int nch) { return 3 * nch * CHUNK; }
-__host__ __device__ constexpr int off_misc(int nch) { return 3 * nch * CHUNK + (nch == 9 ? 0 : 3 * P_BYTES); }
-__host__ __device__ constexpr int smem_total(int nch) { return off_misc(nch) + MISC_BYTES + 1024; }
+//
+// E4M3 cache (e8): the same ring with TWO frames of bf16 chunks, and two STAGES in front of it, each a whole
+// quantised page as it lies in the pool (scales, rope plane, codes: one contiguous block).  Four warps turn a
+// stage into a frame, chunk by chunk; from the frame on nothing differs.  A frame is no longer held
+// while its copy is on the way (that is the stage's part, at little more than half the bytes), so two of them
+// do what three did.
+__host__ __device__ constexpr int n_frames(bool e8) { return e8 ? 2 : 3; }
+constexpr int E8_SCALES = TILE * 8, E8_CODES_OFF = E8_SCALES + CHUNK, E8_GROUP = TILE * 64;  // within a page: 512 B | 8 KB rope | 4 KB per group
+__host__ __device__ constexpr int e8_page(int nch) { return E8_CODES_OFF + (nch - 1) * E8_GROUP; }
+constexpr int E8_PIECE0 = E8_CODES_OFF + 3 * E8_GROUP;  // scales, rope and three groups land first
+__host__ __device__ constexpr int off_pbuf(int nch, bool e8) { return n_frames(e8) * nch * CHUNK; }
+__host__ __device__ constexpr int off_stage(int nch, bool e8) { return off_pbuf(nch, e8) + (nch == 9 ? 0 : n_frames(e8) * P_BYTES); }
+__host__ __device__ constexpr int off_misc(int nch, bool e8) { return off_stage(nch, e8) + (e8 ? 2 * e8_page(nch) : 0); }
+// (with stages nothing is left to align the base by hand: the kernel checks it)
+__host__ __device__ constexpr int smem_total(int nch, bool e8) { return off_misc(nch, e8) + MISC_BYTES + (e8 ? 0 : 1024); }
 // byte offset (from the ring base) of the P buffer of the tile in ring slot g
-template <int NCH>
+template <int NCH, bool E8>
 __device__ __forceinline__ int p_slot_off(int g) {
-  return NCH == 9 ? ((g % 3) * NCH + 8) * CHUNK : off_pbuf(NCH) + (g % 3) * P_BYTES;
+  constexpr int F = n_frames(E8);
+  return NCH == 9 ? ((g % F) * NCH + 8) * CHUNK : off_pbuf(NCH, E8) + (g % F) * P_BYTES;
 }
 
 struct StreamParams {
@@ -74,7 +88,8 @@ struct StreamParams {
   const int32_t* tables;
   const AttnSeg* segs;
   const int32_t* cta_seg;
-  const bf16* pool;
+  const unsigned char* pool;  // E4M3: the pages, page_bytes apart
+  long long page_bytes;
   float* part_m;
   float* part_l;
   float* part_o;
@@ -103,6 +118,8 @@ struct StreamMisc {
                          // scores of tile n, barrier n % 3 -- one per buffer, as the QK MMAs may run three tiles ahead
   uint64_t s_free[3];    // the softmax threads have read the partial in this score buffer
   uint64_t p_full[3];    // the probabilities of tile n are written: barrier n % 3
+  uint64_t st_full[2][2];  // E4M3: the two pieces of tile n's page are in stage n & 1
+  uint64_t st_free[2];     // E4M3: stage n & 1 has been dequantised
   uint32_t tmem_slot;
   int abort_flag;
   float pmax[2][2][HEADS];  // [tile parity][token half][head]: row maxima of the two warps of a quadrant
@@ -278,6 +295,12 @@ __device__ __forceinline__ void finish_token(const StreamParams& p, int tok, int
   }
 }
 
+__device__ __forceinline__ void bulk_load_hint(void* dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;"
+               ::"r"(tc::smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(tc::smem_u32(bar)), "l"(policy)
+               : "memory");
+}
+
 // A barrier wait of a whole warp: all lanes go on, or none.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* d_status, int code) {
   return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_flag, d_status, code));
@@ -324,25 +347,37 @@ __device__ __forceinline__ bool qk_chunks(StreamMisc* mi, int g, uint32_t d, uin
 // waiting for it to free a buffer -- the better trade when tiles come from L2 (blocks of query
 // tokens: the kernel is bound by its own pipeline there; attention of the 32 x 16 x 16384 verify block
 // 1.69 -> 1.55 ms), the worse one when the life of a frame bounds the kernel (decode: 86 -> 88 us).
-template <int NCH, bool DIRECT, bool WHOLE, bool FLAT>
-__global__ void __launch_bounds__(ST_THREADS, 1)
+// E8: the cache is held in E4M3 (cache_rows.cuh).
+template <int NCH, bool DIRECT, bool WHOLE, bool FLAT, bool E8>
+__global__ void __launch_bounds__(E8 ? E8_THREADS : ST_THREADS, 1)
 k_attn_stream(const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ CUtensorMap tmQ, StreamParams p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* s_ring = smem;
-  StreamMisc* mi = reinterpret_cast<StreamMisc*>(smem + off_misc(NCH));
+  StreamMisc* mi = reinterpret_cast<StreamMisc*>(smem + off_misc(NCH, E8));
+  constexpr int F = n_frames(E8), W_QK1 = E8 ? 10 : 13, W_SV = E8 ? 11 : 12;
   volatile int* abort_flag = &mi->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (E8 && smem != smem_raw) {  // (dynamic shared memory starts 1024-byte aligned where a kernel has no static one)
+    if (threadIdx.x == 0) atomicCAS(p.d_status, 0, ST_SMEM_BASE);
+    return;
+  }
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 4; ++i) {
-      for (int j = 0; j < 3; ++j) tc::mbar_init(&mi->full_t[i][j], j < 2 ? 3 : NCH - 6);
+      for (int j = 0; j < 3; ++j) tc::mbar_init(&mi->full_t[i][j], E8 ? 4 : j < 2 ? 3 : NCH - 6);
       tc::mbar_init(&mi->o_done[i], 1);
     }
     tc::mbar_init(&mi->q_ready, 256);
     for (int i = 0; i < 3; ++i) tc::mbar_init(&mi->s_full[i], WHOLE ? 1 : 2);
     for (int i = 0; i < 3; ++i) tc::mbar_init(&mi->s_free[i], 256);
     for (int i = 0; i < 3; ++i) tc::mbar_init(&mi->p_full[i], 256);
+    if (E8)
+      for (int i = 0; i < 2; ++i) {
+        tc::mbar_init(&mi->st_full[i][0], 1);
+        tc::mbar_init(&mi->st_full[i][1], 1);
+        tc::mbar_init(&mi->st_free[i], 4);
+      }
     mi->abort_flag = 0;
     tc::fence_barrier_init();
   }
@@ -359,8 +394,8 @@ k_attn_stream(const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ 
   int page = cur.done() ? 0 : cur.page(p);
   pdl_wait();  // Q_eff and the appended cache rows come from earlier kernels
 
-  if (warp == 0 || warp == 10 || warp == 11) {
-    // ---------------- TMA producers: warps 0, 10, 11 (one elected lane each) ----------------
+  if (warp == 0 || (!E8 && (warp == 10 || warp == 11))) {
+    // ---------------- TMA producers: warps 0, 10, 11 (one elected lane each); E8: warp 0 ----------------
     // Tile g goes to ring frame g % 3, which is free once the SV MMAs of tile g-3 have retired;
     // chunk c of the tile is copied by producer (g * NCH + c) % 3.  The chunks of a tile land in three groups (one
     // chunk of each producer per group), each with its own barrier, so that the QK MMAs of the
@@ -368,7 +403,7 @@ k_attn_stream(const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ 
     {
       const int r = warp == 0 ? 0 : warp - 9;
       if (r == 0 && lane == 0) {
-        tc::tma_prefetch_desc(&tmKV);
+        if (!E8) tc::tma_prefetch_desc(&tmKV);
         tc::tma_prefetch_desc(&tmQ);
       }
       // cache tiles are read once and are more than L2 holds: they leave L2 first, so that the
@@ -393,7 +428,22 @@ k_attn_stream(const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ 
         __syncwarp();
         return true;
       };
-      while (!cur.done()) {
+      while (E8 && !cur.done()) {  // pages into the stages; the Q_eff blocks go from warp 1 straight to their frames
+        const int n = cur.n, b = n & 1;
+        if (n >= 2 && !warp_wait(&mi->st_free[b], ((n >> 1) - 1) & 1, abort_flag, p.d_status, ST_TMA_TIMEOUT)) break;
+        if (tc::elect_one()) {
+          const unsigned char* src = p.pool + page * p.page_bytes;
+          unsigned char* dst = smem + off_stage(NCH, E8) + b * e8_page(NCH);
+          tc::mbar_expect_tx(&mi->st_full[b][0], E8_PIECE0);
+          bulk_load_hint(dst, src, E8_PIECE0, &mi->st_full[b][0], stream_policy);
+          tc::mbar_expect_tx(&mi->st_full[b][1], e8_page(NCH) - E8_PIECE0);
+          bulk_load_hint(dst + E8_PIECE0, src + E8_PIECE0, e8_page(NCH) - E8_PIECE0, &mi->st_full[b][1], stream_policy);
+        }
+        __syncwarp();
+        cur.next(p);
+        if (!cur.done()) page = cur.page(p);
+      }
+      while (!E8 && !cur.done()) {
         // a segment opens with the Q_eff block of its token (64 rows of q_eff)
         if (cur.t == 0 && !fill(cur.gq, &tmQ, cur.sg.tok * HEADS)) break;
         if (!fill(cur.g, &tmKV, page * TILE)) break;
@@ -401,7 +451,7 @@ k_attn_stream(const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ 
         if (!cur.done()) page = cur.page(p);
       }
     }
-  } else if (warp == 1 || warp == 13) {
+  } else if (warp == 1 || warp == W_QK1) {
     // ---------------- QK issuers ----------------
     // A thread needs a few hundred cycles per barrier it waits on and 30 per MMA, so the 36 QK MMAs of a
     // tile are split: warp 1 accumulates chunks 0-4 and warp 13 chunks 5-8 into score buffers of
@@ -414,9 +464,27 @@ k_attn_stream(const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ 
       bool ok = true;
       while (!cur.done() && ok) {
         const int g = cur.g, n = cur.n;
+        if (E8 && part == 0 && cur.t == 0) {
+          // the Q_eff block of the segment's token goes to its frame like a tile of a bf16 cache
+          const int gq = cur.gq;
+          if (gq >= F) ok = warp_wait(&mi->o_done[(gq - F) & 3], ((gq - F) >> 2) & 1, abort_flag, p.d_status, ST_TMA_TIMEOUT);
+          if (ok && tc::elect_one()) {
+            const uint64_t policy = tc::l2_policy_evict_normal();
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+              uint64_t* bar = &mi->full_t[gq & 3][i];  // four arrivals, as the dequantising warps make of a tile's
+              tc::mbar_expect_tx(bar, (i < 2 ? 3 : NCH - 6) * CHUNK);
+              for (int a = 0; a < 3; ++a) tc::mbar_arrive(bar);
+#pragma unroll
+              for (int c = 3 * i; c < 3 * i + 3 && c < NCH; ++c)
+                tc::tma_load_3d_hint(s_ring + ((gq % F) * NCH + c) * CHUNK, &tmQ, bar, c * 64, cur.sg.tok * HEADS, 0, policy);
+            }
+          }
+          __syncwarp();
+        }
         // both issuers wait for Q_eff of every segment; all softmax threads have read the block's
         // frame by then, which is what the producers wait for before they reuse it
-        if (cur.t == 0) {
+        if (ok && cur.t == 0) {
           ok = warp_wait(&mi->q_ready, cur.sidx & 1, abort_flag, p.d_status, ST_MMA_TIMEOUT);
           if (ok && part == 0 && lane == 0) tc::mbar_arrive(&mi->o_done[cur.gq & 3]);
         }
@@ -430,7 +498,7 @@ k_attn_stream(const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ 
         if (!ok) break;
         tc::tc_fence_after();
         const uint32_t d = tmem + COL_S + buf * TILE;  // same lanes as the TMEM-resident A
-        const uint32_t frame16 = ring16 + (g % 3) * NCH * (CHUNK / 16);
+        const uint32_t frame16 = ring16 + (g % F) * NCH * (CHUNK / 16);
         if (WHOLE) ok = qk_chunks<0, NCH>(mi, g, d, tmem, frame16, abort_flag, p.d_status);
         else if (part == 0) ok = qk_chunks<0, 5>(mi, g, d, tmem, frame16, abort_flag, p.d_status);
         else ok = qk_chunks<5, NCH>(mi, g, d, tmem, frame16, abort_flag, p.d_status);
@@ -440,7 +508,7 @@ k_attn_stream(const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ 
         cur.next(p);
       }
     }
-  } else if (warp == 12) {
+  } else if (warp == W_SV) {
     // ---------------- SV issuer ----------------
     {
       const uint64_t k_major = tc::umma_desc_sw128(0, 16, 1024);
@@ -451,20 +519,70 @@ k_attn_stream(const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ 
         const int g = cur.g;
         if (!warp_wait(&mi->p_full[cur.n % 3], (cur.n / 3) & 1, abort_flag, p.d_status, ST_MMA_TIMEOUT)) break;
         tc::tc_fence_after();
-        const uint64_t da = k_major | (uint64_t)(ring16 + (p_slot_off<NCH>(g) >> 4));
+        const uint64_t da = k_major | (uint64_t)(ring16 + (p_slot_off<NCH, E8>(g) >> 4));
         const uint32_t acc0 = cur.t > 0 ? 1u : 0u;
         if (tc::elect_one()) {
 #pragma unroll
           for (int nh = 0; nh < 2; ++nh) {
             // latent columns 256*nh .. +255 are chunks 4nh .. 4nh+3 of the tile's frame
             const uint32_t d = tmem + LANE16 + COL_O + nh * 256;
-            const uint64_t db = v_desc | (uint64_t)(ring16 + ((g % 3) * NCH + 4 * nh) * (CHUNK / 16));
+            const uint64_t db = v_desc | (uint64_t)(ring16 + ((g % F) * NCH + 4 * nh) * (CHUNK / 16));
 #pragma unroll
             for (int k = 0; k < TILE / 16; ++k) tc::umma_bf16(d, da + k * 2, db + k * 128, id256, k > 0 ? 1u : acc0);
           }
           tc::umma_commit(&mi->o_done[g & 3]);
         }
         __syncwarp();
+        cur.next(p);
+      }
+    }
+  } else if (warp >= 12) {
+    // ---------------- E8: stages -> frames (warps 12-15, one on each scheduler) ----------------
+    // A thread has a quarter (16 codes) of two tokens' rows in every group.  Reads of a warp are 512 contiguous bytes;
+    // its stores of 16 bytes meet eight different units of the 128-byte swizzle per eight lanes: no bank is
+    // met twice in either.
+    if constexpr (E8) {
+      const int ct = threadIdx.x - 12 * 32, tk = ct >> 2, qd = ct & 3;
+      while (!cur.done()) {
+        const int g = cur.g, n = cur.n;
+        // the frame is free once the SV MMAs of the slot F back have retired
+        if (g >= F && !warp_wait(&mi->o_done[(g - F) & 3], ((g - F) >> 2) & 1, abort_flag, p.d_status, ST_DEQ_TIMEOUT)) break;
+        if (!warp_wait(&mi->st_full[n & 1][0], (n >> 1) & 1, abort_flag, p.d_status, ST_DEQ_TIMEOUT)) break;
+        const unsigned char* stage = smem + off_stage(NCH, E8) + (n & 1) * e8_page(NCH);
+        unsigned char* frame = s_ring + (g % F) * (NCH * CHUNK);
+        const uint2 sb[2] = {*reinterpret_cast<const uint2*>(stage + tk * 8), *reinterpret_cast<const uint2*>(stage + (tk + 32) * 8)};
+        bool ok = true;
+#pragma unroll 1
+        for (int c = 0; c < NCH - 1; ++c) {
+          if (c == 3) ok = warp_wait(&mi->st_full[n & 1][1], (n >> 1) & 1, abort_flag, p.d_status, ST_DEQ_TIMEOUT);
+          if (!ok) break;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int t = tk + 32 * i;
+            const uint4 w4 = *reinterpret_cast<const uint4*>(stage + E8_CODES_OFF + c * E8_GROUP + t * 64 + qd * 16);
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+            uint2 o[4];
+            e4m3_dequant<4>(w, ((c < 4 ? sb[i].x : sb[i].y) >> (8 * (c & 3))) & 255u, o);
+            unsigned char* dst = frame + c * CHUNK + t * 128;
+            *reinterpret_cast<uint4*>(dst + (((2 * qd) ^ (t & 7)) * 16)) = make_uint4(o[0].x, o[0].y, o[1].x, o[1].y);
+            *reinterpret_cast<uint4*>(dst + (((2 * qd + 1) ^ (t & 7)) * 16)) = make_uint4(o[2].x, o[2].y, o[3].x, o[3].y);
+          }
+          if (c == NCH - 2) {  // the rope dims as they are, in the swizzle of the other chunks
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int t = (ct >> 3) + 16 * i, u = ct & 7;
+              *reinterpret_cast<uint4*>(frame + (NCH - 1) * CHUNK + t * 128 + ((u ^ (t & 7)) * 16)) =
+                  *reinterpret_cast<const uint4*>(stage + E8_SCALES + t * 128 + u * 16);
+            }
+          }
+          if (c == 2 || c == 5 || c == NCH - 2) {
+            tc::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&mi->full_t[g & 3][c == 2 ? 0 : c == 5 ? 1 : 2]);
+          }
+        }
+        if (!ok) break;
+        if (lane == 0) tc::mbar_arrive(&mi->st_free[n & 1]);  // (behind the last __syncwarp: the stage has been read)
         cur.next(p);
       }
     }
@@ -485,7 +603,7 @@ k_attn_stream(const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ 
     auto write_q = [&](int gq) -> bool {
       for (int i = 0; i < 3; ++i)
         if (!tc::mbar_wait(&mi->full_t[gq & 3][i], (gq >> 2) & 1, abort_flag, p.d_status, ST_SOFTMAX_TIMEOUT)) return false;
-      const unsigned char* frame = s_ring + (gq % 3) * (NCH * CHUNK);
+      const unsigned char* frame = s_ring + (gq % F) * (NCH * CHUNK);
       // head `row`, dims 256*half + 128*gsel + 64*sub .. +63: row `row` of chunk 4*half + 2*gsel + sub
       // (128 bytes, eight 16-byte units, unit u at position u ^ (row & 7))
 #pragma unroll
@@ -583,7 +701,7 @@ k_attn_stream(const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ 
           // the QK MMAs of this tile (retired: s_full) were the last to read; with eight it was last
           // read by the SV MMAs of the tile three slots back, which retired before this frame was
           // filled.
-          unsigned char* prow = s_ring + p_slot_off<NCH>(g) + row * 128;
+          unsigned char* prow = s_ring + p_slot_off<NCH, E8>(g) + row * 128;
           const int u0 = half * 4 + sub * 2;
           *reinterpret_cast<uint4*>(prow + (((u0) ^ (row & 7)) * 16)) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
           *reinterpret_cast<uint4*>(prow + (((u0 + 1) ^ (row & 7)) * 16)) = make_uint4(packed[4], packed[5], packed[6], packed[7]);
@@ -662,30 +780,36 @@ k_attn_stream(const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ 
 
 
 bool attn_stream_supported(const AttnArgs& a) {
-  return a.H == HEADS && a.d_v == D_V && a.page_tokens == TILE && a.row == a.d_qk &&
+  return a.H == HEADS && a.d_v == D_V && a.page_tokens == TILE && a.pool.row == a.d_qk &&
          (a.d_qk == 576 || a.d_qk == 512) && a.pool_rows < (1ll << 31) &&
-         (reinterpret_cast<uintptr_t>(a.pool) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.q_eff) & 15) == 0;
+         // E4M3 pages have to be the stages' (64 rope dims, the codes of eight or seven groups behind them)
+         (!a.pool.e4m3 || (a.pool.rope == 64 && a.pool.page_bytes == e8_page(a.d_qk / 64))) &&
+         (reinterpret_cast<uintptr_t>(a.pool.base) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.q_eff) & 15) == 0;
 }
 
 cudaError_t launch_attn_stream(const AttnArgs& a, cudaStream_t st) {
   static_assert(sizeof(StreamMisc) <= MISC_BYTES, "misc region too small");
-  static_assert(smem_total(9) <= 227 * 1024 && smem_total(8) <= 227 * 1024, "shared memory budget");
+  static_assert(smem_total(9, false) <= 227 * 1024 && smem_total(8, false) <= 227 * 1024, "shared memory budget");
+  static_assert(smem_total(9, true) <= 227 * 1024 && smem_total(8, true) <= 227 * 1024, "shared memory budget");
+  static_assert(E8_PIECE0 % 16 == 0 && e8_page(9) % 128 == 0 && e8_page(8) % 128 == 0, "bulk copies and bf16 rope rows");
   static_assert(COL_S + 3 * TILE <= TMEM_COLS, "tensor memory budget");
   if (a.n_segs <= 0 && a.flat_rows <= 0) return cudaSuccess;
-  CUtensorMap tmKV;
   const char* err = nullptr;
-  if (!tc::cached_tmap(&tmKV, a.pool, (uint64_t)a.row, (uint64_t)a.pool_rows, 1, (uint64_t)a.row * 2,
-                       (uint64_t)a.row * 2 * (uint64_t)a.pool_rows, 64, TILE, 1, &err))
-    return cudaErrorInvalidValue;
-  // Q_eff has the geometry of the pool: rows of d_qk values, a token's 64 heads are one "page"
+  // Q_eff has the geometry of a bf16 pool: rows of d_qk values, a token's 64 heads are one "page"
   CUtensorMap tmQ;
   if (!tc::cached_tmap(&tmQ, a.q_eff, (uint64_t)a.d_qk, (uint64_t)a.q_rows, 1, (uint64_t)a.d_qk * 2,
                        (uint64_t)a.d_qk * 2 * (uint64_t)a.q_rows, 64, HEADS, 1, &err))
     return cudaErrorInvalidValue;
+  CUtensorMap tmKV = tmQ;  // (E4M3: not read)
+  if (!a.pool.e4m3 &&
+      !tc::cached_tmap(&tmKV, a.pool.base, (uint64_t)a.pool.row, (uint64_t)a.pool_rows, 1, (uint64_t)a.pool.row * 2,
+                       (uint64_t)a.pool.row * 2 * (uint64_t)a.pool_rows, 64, TILE, 1, &err))
+    return cudaErrorInvalidValue;
   StreamParams p;
   p.q_eff = a.q_eff; p.tables = a.tables; p.segs = a.segs; p.cta_seg = a.cta_seg;
   p.part_m = a.part_m; p.part_l = a.part_l; p.part_o = a.part_o; p.d_status = a.d_status;
-  p.pool = a.pool;
+  p.pool = a.pool.base;
+  p.page_bytes = a.pool.page_bytes;
   p.d_qk = a.d_qk;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.direct = a.direct_single ? 1 : 0;
@@ -694,15 +818,17 @@ cudaError_t launch_attn_stream(const AttnArgs& a, cudaStream_t st) {
   p.tiles_shared = a.tiles_shared ? 1 : 0;
   p.flat_rows = a.flat_rows;
   const bool whole = a.tiles_shared;
-#define FST_ATTN_LAUNCH(NCHV, DIR, WH, FL) \
-  launch_k(a.dependent_launch, k_attn_stream<NCHV, DIR, WH, FL>, dim3(a.n_ctas), dim3(ST_THREADS), smem_total(NCHV), st, 1, tmKV, tmQ, p)
-  if (a.flat_rows > 0) return a.d_qk == 576 ? FST_ATTN_LAUNCH(9, false, false, true) : FST_ATTN_LAUNCH(8, false, false, true);
-  if (a.d_qk == 576) {
-    if (whole) return p.direct ? FST_ATTN_LAUNCH(9, true, true, false) : FST_ATTN_LAUNCH(9, false, true, false);
-    return p.direct ? FST_ATTN_LAUNCH(9, true, false, false) : FST_ATTN_LAUNCH(9, false, false, false);
-  }
-  if (whole) return p.direct ? FST_ATTN_LAUNCH(8, true, true, false) : FST_ATTN_LAUNCH(8, false, true, false);
-  return p.direct ? FST_ATTN_LAUNCH(8, true, false, false) : FST_ATTN_LAUNCH(8, false, false, false);
+#define FST_ATTN_LAUNCH(NCHV, DIR, WH, FL, E8V)                                                                             \
+  launch_k(a.dependent_launch, k_attn_stream<NCHV, DIR, WH, FL, E8V>, dim3(a.n_ctas), dim3(E8V ? E8_THREADS : ST_THREADS), \
+           smem_total(NCHV, E8V), st, 1, tmKV, tmQ, p)
+#define FST_ATTN_PICK(NCHV, E8V)                                                                                     \
+  (whole ? p.direct ? FST_ATTN_LAUNCH(NCHV, true, true, false, E8V) : FST_ATTN_LAUNCH(NCHV, false, true, false, E8V) \
+         : p.direct ? FST_ATTN_LAUNCH(NCHV, true, false, false, E8V) : FST_ATTN_LAUNCH(NCHV, false, false, false, E8V))
+  if (a.flat_rows > 0)
+    return a.d_qk == 576 ? FST_ATTN_LAUNCH(9, false, false, true, false) : FST_ATTN_LAUNCH(8, false, false, true, false);
+  if (a.pool.e4m3) return a.d_qk == 576 ? FST_ATTN_PICK(9, true) : FST_ATTN_PICK(8, true);
+  return a.d_qk == 576 ? FST_ATTN_PICK(9, false) : FST_ATTN_PICK(8, false);
+#undef FST_ATTN_PICK
 #undef FST_ATTN_LAUNCH
 }
 

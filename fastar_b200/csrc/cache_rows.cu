@@ -1,0 +1,134 @@
+// Rows into and out of the paged cache: append of given rows, read-back, and the page copies and
+// zeroing of forked and truncated sequences, for the bf16 and the E4M3 format (cache_rows.cuh).
+//
+// All of them move each row once and compute next to nothing: bound by bytes for long runs, by the launch
+// for a decode step's few rows.  A warp per row, 16 bytes of bf16 per lane; the maximum of a group
+// of 64 values is three shuffles among the eight lanes that hold it, so a row is quantised in registers
+// between its load and its store.
+#include "kernels.cuh"
+
+namespace fst {
+
+namespace {
+
+constexpr int ROW_WARPS = 4;   // few rows then still spread over the SMs: 64 rows are 16 blocks
+constexpr int MAX_PASS = 4;    // row <= 1024: units of eight values per lane
+
+__device__ __forceinline__ void copy_in(const PoolView& v, long long r, const bf16* src, int lane) {
+  const int units = v.row / 8;
+  uint4 x[MAX_PASS];
+#pragma unroll
+  for (int i = 0; i < MAX_PASS; ++i)
+    if (i * 32 + lane < units) x[i] = reinterpret_cast<const uint4*>(src)[i * 32 + lane];
+#pragma unroll
+  for (int i = 0; i < MAX_PASS; ++i)
+    if (i * 32 < units) store_unit(v, r, i * 32 + lane, x[i], i * 32 + lane < units);
+}
+
+// Row t of `rows` -> pool row dst[t] (-1: the row is not kept).
+__global__ void __launch_bounds__(ROW_WARPS * 32) k_rows_append(PoolView v, const bf16* rows, const long long* dst, int T) {
+  pdl_launch();
+  const int t = blockIdx.x * ROW_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  pdl_wait();
+  if (t >= T) return;
+  const long long d = dst[t];
+  if (d < 0) return;
+  copy_in(v, v.e4m3 ? d : d / v.row, rows + (long long)t * v.row, lane);
+}
+
+// Runs of rows that are neighbours in the pool and in the buffer; WRITE: buffer -> pool, else pool -> buffer.
+template <bool WRITE>
+__global__ void __launch_bounds__(ROW_WARPS * 32) k_rows_runs(PoolView v, bf16* buf, RowRuns inl, const RowRun* runs) {
+  pdl_launch();
+  const int i = blockIdx.x * ROW_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  pdl_wait();
+  const RowRun run = runs ? runs[blockIdx.y] : inl.run[blockIdx.y];
+  if (i >= run.n) return;
+  const long long r = (long long)run.pool_row + i;
+  bf16* b = buf + (long long)(run.buf_row + i) * v.row;
+  if (WRITE) {
+    copy_in(v, r, b, lane);
+  } else {
+    const int units = v.row / 8;
+    uint4 x[MAX_PASS];
+#pragma unroll
+    for (int k = 0; k < MAX_PASS; ++k)
+      if (k * 32 + lane < units) x[k] = load_unit(v, r, k * 32 + lane);
+#pragma unroll
+    for (int k = 0; k < MAX_PASS; ++k)
+      if (k * 32 + lane < units) reinterpret_cast<uint4*>(b)[k * 32 + lane] = x[k];
+  }
+}
+
+// Slots [0, keep) of page `src` -> page `dst`, zeros behind them.  Bits are moved as they are held.
+// (Zeros, not what the source has there: a masked row is multiplied by a probability of 0.)
+__global__ void __launch_bounds__(256) k_page_copy(PoolView v, int src, int dst, int keep) {
+  pdl_launch();
+  pdl_wait();
+  const unsigned char* s = v.base + src * v.page_bytes;
+  unsigned char* d = v.base + dst * v.page_bytes;
+  const int step = gridDim.x * blockDim.x, t0 = blockIdx.x * blockDim.x + threadIdx.x;
+  // a plane of pt pieces of `w` bytes (a multiple of 8), the first `keep` of them kept
+  auto plane = [&](long long off, int w) {
+    const long long n = (long long)v.pt * w / 8, k = (long long)keep * w / 8;
+    for (long long i = t0; i < n; i += step)
+      reinterpret_cast<uint2*>(d + off)[i] = i < k ? reinterpret_cast<const uint2*>(s + off)[i] : make_uint2(0, 0);
+  };
+  if (!v.e4m3) {
+    plane(0, v.row * 2);
+    return;
+  }
+  plane(0, v.sp);
+  plane(v.off_rope, v.rope * 2);
+  for (int g = 0; g * E4M3_GROUP < v.n8; ++g)
+    plane(v.off_codes + (long long)g * v.pt * E4M3_GROUP, min(E4M3_GROUP, v.n8 - g * E4M3_GROUP));
+}
+
+// Zero whole cache rows (speculative rollback, reference src/fst_engine.cpp:6132-6147) of an E4M3 pool.
+__global__ void __launch_bounds__(128) k_rows_zero_e4m3(PoolView v, const long long* rows) {
+  const int r = (int)rows[blockIdx.x], pg = r / v.pt, s = r - pg * v.pt;
+  unsigned char* page = v.base + pg * v.page_bytes;
+  for (int u = threadIdx.x; u < v.row / 8; u += blockDim.x) {
+    if (u * 8 >= v.n8) {
+      *reinterpret_cast<uint4*>(page + v.off_rope + ((long long)s * v.rope + u * 8 - v.n8) * 2) = make_uint4(0, 0, 0, 0);
+    } else {
+      *reinterpret_cast<uint2*>(page + e4m3_code_off(v, s, u)) = make_uint2(0, 0);
+      if ((u & 7) == 0) page[s * v.sp + (u >> 3)] = 0;
+    }
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_rows_append(const PoolView& v, const bf16* rows, const long long* dst, int T, cudaStream_t st) {
+  if (T <= 0) return cudaSuccess;
+  return launch_pdl(k_rows_append, dim3((T + ROW_WARPS - 1) / ROW_WARPS), dim3(ROW_WARPS * 32), 0, st, 1, v, rows, dst, T);
+}
+
+cudaError_t launch_rows_runs(const PoolView& v, bf16* buf, const RowRun* host_runs, const RowRun* dev_runs, int n_runs, int max_n,
+                             bool write, cudaStream_t st) {
+  if (n_runs <= 0 || max_n <= 0) return cudaSuccess;
+  const unsigned gx = (unsigned)((max_n + ROW_WARPS - 1) / ROW_WARPS);
+  for (int r0 = 0; r0 < n_runs; r0 += 65535) {  // (a grid has at most 65535 blocks along y)
+    const int n = n_runs - r0 < 65535 ? n_runs - r0 : 65535;
+    RowRuns inl;
+    if (!dev_runs)
+      for (int i = 0; i < n; ++i) inl.run[i] = host_runs[i];  // (at most RowRuns::CAP, the caller's duty)
+    const RowRun* dev = dev_runs ? dev_runs + r0 : nullptr;
+    cudaError_t e = write ? launch_pdl(k_rows_runs<true>, dim3(gx, n), dim3(ROW_WARPS * 32), 0, st, 1, v, buf, inl, dev)
+                          : launch_pdl(k_rows_runs<false>, dim3(gx, n), dim3(ROW_WARPS * 32), 0, st, 1, v, buf, inl, dev);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+cudaError_t launch_page_copy(const PoolView& v, int src, int dst, int keep, cudaStream_t st) {
+  return launch_pdl(k_page_copy, dim3(8), dim3(256), 0, st, 1, v, src, dst, keep);
+}
+
+void launch_zero_rows_e4m3(const PoolView& v, const long long* rows, int n_rows, cudaStream_t st) {
+  if (n_rows <= 0) return;
+  k_rows_zero_e4m3<<<n_rows, 128, 0, st>>>(v, rows);
+}
+
+}  // namespace fst

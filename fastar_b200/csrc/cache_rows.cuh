@@ -1,0 +1,163 @@
+// Cache rows in a layer's pool: where a row lives and how it is held, for the bf16 and the E4M3 format.
+//
+// bf16: rows one behind the other, row r of the pool at r * row elements.
+//
+// E4M3: a page of pt rows is one block of three planes,
+//   scales [pt, sp] bytes   one E8M0 byte per group of 64 latent values: 2^(b - 127); 255: the group holds a NaN
+//   rope   [pt, rope] bf16  the rotated dims as they are (they carry the position and are few)
+//   codes  [groups][pt, 64] E4M3 values, group by group: a group of a page (4 KB) is one contiguous
+//                           block, the source of one 64-column chunk of the attention's tile
+// 648 bytes for a 576-wide row instead of 1152, 520 (of 584 allocated: seven scale bytes of eight, pages
+// rounded up) instead of 1024 for a 512-wide one.
+//
+// Quantisation of a group x[64] (bf16 values): a = max |x|; k = the least integer with a <= 448 * 2^k, clamped to
+// [-100, 120]; code = x * 2^-k rounded to E4M3, nearest even (448 is E4M3's largest value: nothing overflows).
+// The scale is a power of two, so code * 2^k has E4M3's four significant bits and IS a bf16 value: what is read
+// back, what the attention multiplies, and what a bf16 cache would hold of the rounded row are the same bits.  The
+// price against a scale of a / 448 is at most one bit of exponent range, none of precision.  At most 1/16 of
+// a value is lost to the rounding, and 2^-10 * 2^k of values below 2^-6 * 2^k.  Magnitudes above 1.875 * 2^127
+// (infinities among them) saturate there: the largest value whose rounding up stays finite in bf16.
+#pragma once
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace fst {
+
+constexpr int E4M3_GROUP = 64;
+
+struct PoolView {
+  unsigned char* base = nullptr;
+  int e4m3 = 0;
+  int row = 0, rope = 0;     // values of a row, rope values among them
+  int pt = 0;                // rows of a page
+  int n8 = 0, sp = 0;        // E4M3: latent values of a row; scale bytes of a row (a multiple of 8)
+  int off_rope = 0, off_codes = 0;  // E4M3: byte offsets of the planes within a page
+  long long page_bytes = 0;
+};
+
+inline PoolView pool_view(void* base, bool e4m3, int row, int rope, int pt) {
+  PoolView v;
+  v.base = static_cast<unsigned char*>(base);
+  v.e4m3 = e4m3;
+  v.row = row;
+  v.rope = rope;
+  v.pt = pt;
+  if (!e4m3) {
+    v.page_bytes = (long long)pt * row * 2;
+    return v;
+  }
+  v.n8 = row - rope;
+  v.sp = ((v.n8 + E4M3_GROUP - 1) / E4M3_GROUP + 7) / 8 * 8;
+  v.off_rope = (pt * v.sp + 127) / 128 * 128;
+  v.off_codes = v.off_rope + (pt * rope * 2 + 127) / 128 * 128;
+  v.page_bytes = (v.off_codes + (long long)pt * v.n8 + 127) / 128 * 128;
+  return v;
+}
+
+// ---- one row, 16 bytes of bf16 (eight values, a "unit") at a time -----------------------------------
+
+// Where the eight codes of unit u of slot s lie within a page (the last group may be narrower than 64).
+__device__ __forceinline__ long long e4m3_code_off(const PoolView& v, int s, int u) {
+  const int g = u >> 3, width = min(E4M3_GROUP, v.n8 - g * E4M3_GROUP);
+  return v.off_codes + (long long)g * v.pt * E4M3_GROUP + s * width + (u & 7) * 8;
+}
+
+// The scale byte of a group from the largest |x| of it, given as the bits of an fp32 value (a NaN's are
+// larger than every number's).
+__device__ __forceinline__ int e4m3_scale_byte(uint32_t amax_bits) {
+  if (amax_bits > 0x7F800000u) return 255;
+  amax_bits = min(amax_bits, 0x7F700000u);  // 1.875 * 2^127
+  // a = m * 2^e with 1 <= m < 2; 448 = 1.75 * 2^8
+  const int k = (int)(amax_bits >> 23) - 127 - 8 + ((amax_bits & 0x7FFFFFu) > 0x600000u);
+  return max(-100, min(120, k)) + 127;
+}
+// Eight bf16 values -> eight codes under the scale byte b.
+__device__ __forceinline__ uint2 e4m3_quant8(uint4 x, int b) {
+  const float inv = __uint_as_float((uint32_t)(254 - min(b, 247)) << 23);  // 2^-k
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  uint32_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float top = __uint_as_float(0x7F700000u);
+    float2 f = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+    f.x = fminf(fmaxf(f.x, -top), top) * inv;
+    f.y = fminf(fmaxf(f.y, -top), top) * inv;
+    h[i] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+  }
+  return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+}
+
+// Four codes -> four bf16 values.  A code's bits moved to where bf16 has exponent and fraction are the value
+// times 2^-120 (bias 127 against 7; E4M3's subnormals land on bf16's); one multiplication by 2^(120 + k)
+// puts both right, exactly.  mult: that factor; beyond b = 134 it is no bf16 value, see e4m3_dequant.
+__device__ __forceinline__ uint2 e4m3_to_bf16x4(uint32_t w, __nv_bfloat162 mult) {
+  const uint32_t a = __byte_perm(w, 0, 0x1404), b = __byte_perm(w, 0, 0x3424);
+  const uint32_t ra = ((a >> 4) & 0x07F007F0u) | (a & 0x80008000u), rb = ((b >> 4) & 0x07F007F0u) | (b & 0x80008000u);
+  const __nv_bfloat162 ya = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&ra), mult);
+  const __nv_bfloat162 yb = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&rb), mult);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&ya), *reinterpret_cast<const uint32_t*>(&yb));
+}
+__device__ __forceinline__ __nv_bfloat162 bf162_of_bits(uint32_t bits16) {
+  const uint32_t w = bits16 | (bits16 << 16);
+  return *reinterpret_cast<const __nv_bfloat162*>(&w);
+}
+// N words of four codes each, under the scale byte b.
+template <int N>
+__device__ __forceinline__ void e4m3_dequant(const uint32_t* w, int b, uint2* out) {
+  const __nv_bfloat162 m = bf162_of_bits((uint32_t)(min(b, 134) + 120) << 7);
+#pragma unroll
+  for (int i = 0; i < N; ++i) out[i] = e4m3_to_bf16x4(w[i], m);
+  if (b > 134) {  // groups of values above 57344 (m was 2^127: the rest of the factor), or with a NaN
+    const __nv_bfloat162 m1 = bf162_of_bits(b == 255 ? 0x7FC0u : (uint32_t)(b - 7) << 7);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const __nv_bfloat162 x = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&out[i].x), m1);
+      const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&out[i].y), m1);
+      out[i] = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+    }
+  }
+}
+
+// Unit u (eight values) of pool row r as bf16.
+__device__ __forceinline__ uint4 load_unit(const PoolView& v, long long r, int u) {
+  if (!v.e4m3) return *reinterpret_cast<const uint4*>(v.base + (r * v.row + u * 8) * 2);
+  const int pg = (int)r / v.pt, s = (int)r - pg * v.pt;  // (an E4M3 pool has fewer than 2^31 rows)
+  const unsigned char* page = v.base + pg * v.page_bytes;
+  if (u * 8 >= v.n8) return *reinterpret_cast<const uint4*>(page + v.off_rope + ((long long)s * v.rope + u * 8 - v.n8) * 2);
+  const uint2 c = *reinterpret_cast<const uint2*>(page + e4m3_code_off(v, s, u));
+  const uint32_t w[2] = {c.x, c.y};
+  uint2 o[2];
+  e4m3_dequant<2>(w, page[s * v.sp + (u >> 3)], o);
+  return make_uint4(o[0].x, o[0].y, o[1].x, o[1].y);
+}
+
+// Lane-wise store of unit u of pool row r.  The eight lanes of an aligned group of eight hold the eight units
+// of an aligned group of units (all 32 lanes call it; `on` says whether the lane has a unit at all).
+__device__ __forceinline__ void store_unit(const PoolView& v, long long r, int u, uint4 x, bool on) {
+  if (!v.e4m3) {
+    if (on) *reinterpret_cast<uint4*>(v.base + (r * v.row + u * 8) * 2) = x;
+    return;
+  }
+  const bool latent = on && u * 8 < v.n8;
+  uint32_t a = 0;
+  if (latent) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a = max(a, max((w[i] << 16) & 0x7FFFFFFFu, w[i] & 0x7FFF0000u));
+  }
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+  if (!on) return;
+  const int pg = (int)r / v.pt, s = (int)r - pg * v.pt;
+  unsigned char* page = v.base + pg * v.page_bytes;
+  if (!latent) {
+    *reinterpret_cast<uint4*>(page + v.off_rope + ((long long)s * v.rope + u * 8 - v.n8) * 2) = x;
+    return;
+  }
+  const int b = e4m3_scale_byte(a);
+  *reinterpret_cast<uint2*>(page + e4m3_code_off(v, s, u)) = e4m3_quant8(x, b);
+  if ((u & 7) == 0) page[s * v.sp + (u >> 3)] = (unsigned char)b;
+}
+
+}  // namespace fst

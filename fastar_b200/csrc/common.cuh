@@ -58,6 +58,6 @@ struct AttnSeg {
 
 // Status word values written by kernels that give up a bounded wait.
 enum : int { ST_OK = 0, ST_TMA_TIMEOUT = 1, ST_MMA_TIMEOUT = 2, ST_SOFTMAX_TIMEOUT = 3, ST_EPI_TIMEOUT = 4,
-              ST_SELFTEST_TIMEOUT = 5 };
+              ST_SELFTEST_TIMEOUT = 5, ST_DEQ_TIMEOUT = 6, ST_SMEM_BASE = 7 };
 
 }  // namespace fst

@@ -3,6 +3,7 @@
 #include <map>
 #include <mutex>
 #include <utility>
+#include "cache_rows.cuh"
 #include "common.cuh"
 
 namespace fst {
@@ -133,10 +134,10 @@ struct NormAppendArgs {
   const bf16* q_norm;   // [q_lora] or null
   const bf16* kv_norm;  // [kv_lora] or null
   const float* lut;     // [T, rope] (cos, sin) pairs
-  const long long* dst_row;  // [T] element offset of the cache row in the pool, or -1
+  const long long* dst_row;  // [T] element offset of the cache row in the pool (E4M3 pools: the pool row), or -1
   bf16* qc;             // [T, q_lora]
   bf16* kv_new;         // [T, row]
-  bf16* pool;
+  PoolView pool;
   int T, q_lora, kv_lora, row, rope;
   float eps;
 };
@@ -158,7 +159,7 @@ void launch_q_prep(const QPrepArgs& a, cudaStream_t st);
 
 struct AttnArgs {
   const bf16* q_eff;        // [T * H, d_qk]
-  const bf16* pool;         // [n_pages * page_tokens, row]
+  PoolView pool;            // n_pages * page_tokens rows
   const int32_t* tables;    // flat block tables (a segment names where its table starts)
   const AttnSeg* segs;
   const int32_t* cta_seg;   // [n_ctas + 1] segment ranges of the persistent CTAs
@@ -259,5 +260,21 @@ struct CompressArgs {
 void launch_compress(const CompressArgs& a, cudaStream_t st);
 
 void launch_zero_rows(bf16* pool, const long long* row_off, int n_rows, int row, cudaStream_t st);
+
+// Rows into and out of a pool of either format (cache_rows.cu).
+// dst: [T] element offsets (E4M3 pools: pool rows) as NormAppendArgs::dst_row has them.
+cudaError_t launch_rows_append(const PoolView& v, const bf16* rows, const long long* dst, int T, cudaStream_t st);
+struct RowRun {
+  int32_t pool_row, buf_row, n;  // rows pool_row .. of the pool, buf_row .. of the buffer
+};
+struct RowRuns {  // runs that travel as a kernel argument
+  static constexpr int CAP = 250;
+  RowRun run[CAP];
+};
+// host_runs (at most RowRuns::CAP, passed by value) or dev_runs; max_n: rows of the longest run.
+cudaError_t launch_rows_runs(const PoolView& v, bf16* buf, const RowRun* host_runs, const RowRun* dev_runs, int n_runs, int max_n,
+                             bool write, cudaStream_t st);
+cudaError_t launch_page_copy(const PoolView& v, int src, int dst, int keep, cudaStream_t st);
+void launch_zero_rows_e4m3(const PoolView& v, const long long* rows, int n_rows, cudaStream_t st);
 
 }  // namespace fst

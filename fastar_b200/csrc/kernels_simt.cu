@@ -207,6 +207,7 @@ void launch_rmsnorm_rows(const bf16* x, const bf16* w, bf16* y, int T, int dim, 
 // Every global load of a block (its row of the compressed activations, the norm weights, the RoPE
 // table, the destination) is issued before anything is reduced, and the two sums of squares
 // share one exchange: the kernel is one memory round trip and one block reduction long.
+template <bool E4M3>
 __global__ void __launch_bounds__(256) k_norm_append(NormAppendArgs a) {
   pdl_launch();
   pdl_wait();
@@ -277,7 +278,17 @@ __global__ void __launch_bounds__(256) k_norm_append(NormAppendArgs a) {
   for (int j = tid; j < a.row; j += blockDim.x) {
     const bf16 v = f2bf(s_row[j]);
     a.kv_new[(long long)t * a.row + j] = v;
-    if (dst >= 0) a.pool[dst + j] = v;
+    if (!E4M3 && dst >= 0) reinterpret_cast<bf16*>(a.pool.base)[dst + j] = v;
+  }
+  if (E4M3 && dst >= 0) {  // (the same for the whole block) quantised from the bf16 values, eight per thread
+    for (int u0 = 0; u0 < a.row / 8; u0 += blockDim.x) {
+      const int u = u0 + tid;
+      const bool has = u < a.row / 8;
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = has ? s_row[u * 8 + e] : 0.0f;
+      store_unit(a.pool, dst, u, pack8(x), has);
+    }
   }
 }
 
@@ -289,6 +300,7 @@ __global__ void __launch_bounds__(256) k_norm_append(NormAppendArgs a) {
 // early reads / without, us: V4 two layers of 5 users 210.1 / 212.3, of 2 users 158.4 / 159.6, of one 224.2 /
 // 227.2; BASELINE one row over 131 072 rows 102.4 / 101.8 (on another box 105.2, where the scalar kernel took
 // 102.5), over 4096 74.5 / 74.4.
+template <bool E4M3>
 __global__ void __launch_bounds__(512) k_norm_append_vec(NormAppendArgs a) {
   pdl_launch();
   const bool early = a.row == a.kv_lora;
@@ -326,7 +338,7 @@ __global__ void __launch_bounds__(512) k_norm_append_vec(NormAppendArgs a) {
   __syncthreads();
   ss = warp_sum((is_q ? lane < q_warps : lane >= q_warps && lane < nw) ? scratch[lane] : 0.0f);
   const float r = 1.0f / sqrtf(ss / (float)dim + a.eps);
-  if (!on) return;
+  if (!E4M3 && !on) return;
   if (normed) {
     float g[8];
     unpack8(wv, g);
@@ -344,10 +356,14 @@ __global__ void __launch_bounds__(512) k_norm_append_vec(NormAppendArgs a) {
   }
   const uint4 o = pack8(x);
   if (is_q) {
-    *reinterpret_cast<uint4*>(a.qc + (long long)t * a.q_lora + j0) = o;
+    if (on) *reinterpret_cast<uint4*>(a.qc + (long long)t * a.q_lora + j0) = o;
   } else {
-    *reinterpret_cast<uint4*>(a.kv_new + (long long)t * a.row + j0) = o;
-    if (dst >= 0) *reinterpret_cast<uint4*>(a.pool + dst + j0) = o;
+    if (on) *reinterpret_cast<uint4*>(a.kv_new + (long long)t * a.row + j0) = o;
+    if (E4M3) {
+      if (dst >= 0) store_unit(a.pool, dst, u, o, on);  // (a warp of key units as a whole)
+    } else if (dst >= 0) {
+      *reinterpret_cast<uint4*>(a.pool.base + (dst + j0) * 2) = o;
+    }
   }
 }
 
@@ -358,11 +374,11 @@ void launch_norm_append(const NormAppendArgs& a, cudaStream_t st) {
   // its call.  (A cache row starts at a multiple of `row` elements.)
   const int threads = ((a.q_lora / 8 + 31) / 32 + (a.row / 8 + 31) / 32) * 32;
   if (a.q_lora % 8 == 0 && a.row % 8 == 0 && a.kv_lora % 8 == 0 && a.rope % 8 == 0 && threads <= 512 && aligned16(a.cmp) &&
-      aligned16(a.q_norm) && aligned16(a.kv_norm) && aligned16(a.lut) && aligned16(a.qc) && aligned16(a.kv_new) && aligned16(a.pool)) {
-    launch_pdl(k_norm_append_vec, dim3(a.T), dim3(threads), 0, st, 1, a);
+      aligned16(a.q_norm) && aligned16(a.kv_norm) && aligned16(a.lut) && aligned16(a.qc) && aligned16(a.kv_new) && aligned16(a.pool.base)) {
+    launch_pdl(a.pool.e4m3 ? k_norm_append_vec<true> : k_norm_append_vec<false>, dim3(a.T), dim3(threads), 0, st, 1, a);
     return;
   }
-  launch_pdl(k_norm_append, dim3(a.T), dim3(256), a.row * sizeof(float), st, 1, a);
+  launch_pdl(a.pool.e4m3 ? k_norm_append<true> : k_norm_append<false>, dim3(a.T), dim3(256), a.row * sizeof(float), st, 1, a);
 }
 
 // ---- query preparation -----------------------------------------------------------------------
@@ -515,6 +531,8 @@ void launch_q_prep(const QPrepArgs& a, cudaStream_t st) {
 constexpr int SIMT_TILE = 32;
 constexpr int SIMT_HPW = 8;  // heads per warp
 
+// E4M3: rows are turned into their bf16 values on the way to shared memory; everything behind is the same.
+template <bool E4M3>
 __global__ void __launch_bounds__(256, 1) k_attn_simt(AttnArgs a) {
   pdl_launch();
   pdl_wait();
@@ -550,7 +568,7 @@ __global__ void __launch_bounds__(256, 1) k_attn_simt(AttnArgs a) {
         const int s = min(s0 + rr, seg.kv_end - 1);
         const long long prow = (long long)table[s / a.page_tokens] * a.page_tokens + s % a.page_tokens;
         *reinterpret_cast<uint4*>(s_tile + (size_t)rr * stride + cc * 16) =
-            *reinterpret_cast<const uint4*>(a.pool + prow * a.row + cc * 8);
+            E4M3 ? load_unit(a.pool, prow, cc) : *reinterpret_cast<const uint4*>(a.pool.base + (prow * a.row + cc * 8) * 2);
       }
       __syncthreads();
       // scores: lane = token of the tile
@@ -630,7 +648,7 @@ __global__ void __launch_bounds__(256, 1) k_attn_simt(AttnArgs a) {
 void launch_attn_simt(const AttnArgs& a, cudaStream_t st) {
   if (a.n_segs <= 0) return;
   const size_t smem = (size_t)a.H * a.d_qk * 2 + (size_t)SIMT_TILE * (a.row * 2 + 16);
-  launch_pdl(k_attn_simt, dim3(a.n_segs), dim3(256), smem, st, 1, a);
+  launch_pdl(a.pool.e4m3 ? k_attn_simt<true> : k_attn_simt<false>, dim3(a.n_segs), dim3(256), smem, st, 1, a);
 }
 
 // ---- log-sum-exp merge ---------------------------------------------------------------------

@@ -8,6 +8,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -102,6 +103,7 @@ constexpr int MAX_EVENT_SETS = 256;
 // 25 142 / 148, 32 154 and 162 / 156 and 159, 48 185 and 188 / 183 and 179, 64 223 and 235 / 215 and 217
 // (V4: 1 row 119 / 125, 25 151 / 151, 32 160 and 165 / 159 and 162, 64 229 and 233 / 220).
 constexpr int SMALL_OUT = 32;
+constexpr int ROWS_TMP = 2048;  // rows per turn of a host copy into or out of an E4M3 pool
 
 // Page-locked rows with an address on the device, or (false) neither: without them the output is copied
 // behind the kernels.  The three calls are cudaHostAlloc, cudaHostGetDevicePointer and cudaFreeHost, or
@@ -132,7 +134,14 @@ struct FstMlaCtx {
   int n_sm = 0;
   cudaStream_t stream = nullptr;
   std::vector<LayerW> layers;
-  std::vector<bf16*> pools;  // per layer [n_pages * page_tokens, row]
+  std::vector<bf16*> pools;  // per layer n_pages pages of page_bytes: bf16 [n_pages * page_tokens, row], or E4M3 pages (cache_rows.cuh)
+  bool e4m3 = false;         // the pools hold E4M3 pages
+  size_t page_bytes = 0;
+  bf16* d_rows_tmp = nullptr;  // [ROWS_TMP, row] host rows on their way into or out of an E4M3 pool
+  // runs of rows of a read-back that do not fit a kernel argument: page-locked and device copy
+  RowRun *h_runs = nullptr, *d_runs = nullptr;
+  int runs_cap = 0;
+  cudaEvent_t runs_ev = nullptr;
 
   // paged-cache bookkeeping (host)
   std::vector<int32_t> free_pages, free_seqs;
@@ -339,9 +348,14 @@ int reserve_pages(FstMlaCtx* c, int32_t seq, int32_t n_tokens) {
   return FST_MLA_OK;
 }
 
-long long row_offset(const FstMlaCtx* c, int32_t seq, int32_t pos) {
+// row of a layer's pool that holds row `pos` of the sequence
+long long pool_row(const FstMlaCtx* c, int32_t seq, int32_t pos) {
   const int pt = c->cfg.page_tokens;
-  return ((long long)c->tables[seq][pos / pt] * pt + pos % pt) * c->d.row;
+  return (long long)c->tables[seq][pos / pt] * pt + pos % pt;
+}
+long long row_offset(const FstMlaCtx* c, int32_t seq, int32_t pos) { return pool_row(c, seq, pos) * c->d.row; }
+PoolView view_of(const FstMlaCtx* c, int lid) {
+  return pool_view(c->pools[lid], c->e4m3, c->d.row, c->d.rope, c->cfg.page_tokens);
 }
 
 template <class T>
@@ -427,10 +441,10 @@ GemmArgs plain_gemm(const bf16* A, const bf16* B, bf16* C, int M, int N, int K) 
   return g;
 }
 
-AttnArgs attn_args(FstMlaCtx* c, int lid, const bf16* q_eff, bool may_fuse = false) {
+AttnArgs attn_args(FstMlaCtx* c, int lid, const bf16* q_eff, bool may_fuse, bf16* o_lat) {
   AttnArgs a;
   a.q_eff = q_eff;
-  a.pool = c->pools[lid];
+  a.pool = view_of(c, lid);
   a.tables = c->d_tables;
   const Sched& S = sched_of(c, lid);
   a.segs = S.d_segs;
@@ -453,7 +467,7 @@ AttnArgs attn_args(FstMlaCtx* c, int lid, const bf16* q_eff, bool may_fuse = fal
   if (may_fuse && c->fused_merge && S.n_single_part > 0) {
     a.direct_single = true;
     a.tok_part = S.d_tok_part;
-    a.o_lat = c->d_olat;
+    a.o_lat = o_lat;
     a.sinks = c->d.v4 ? c->layers[lid].sinks : nullptr;
     a.lut = lut_of(c, lid);
     a.rope = c->d.rope;
@@ -464,12 +478,13 @@ AttnArgs attn_args(FstMlaCtx* c, int lid, const bf16* q_eff, bool may_fuse = fal
 
 // *direct (if given; mode-0 callers): the attention kernel has written the o_lat rows of every
 // token that has exactly one partial; the merge that follows skips them.
-int run_attention(FstMlaCtx* c, int lid, const bf16* q_eff, bool* direct = nullptr) {
+// o_lat: where the output rows go (null: the context's own).
+int run_attention(FstMlaCtx* c, int lid, const bf16* q_eff, bool* direct = nullptr, bf16* o_lat = nullptr) {
   if (direct) *direct = false;
   c->status_by_kernel = false;
   c->info_class = class_of(c, lid);
   if (sched_of(c, lid).n_segs == 0) return FST_MLA_OK;
-  AttnArgs a = attn_args(c, lid, q_eff, direct != nullptr);
+  AttnArgs a = attn_args(c, lid, q_eff, direct != nullptr, o_lat ? o_lat : c->d_olat);
   const bool tc_ok = attn_stream_supported(a);
   if (!(c->cfg.attn_impl != FST_MLA_IMPL_SIMT && tc_ok)) a.direct_single = false;
   if (direct) *direct = a.direct_single;
@@ -529,7 +544,7 @@ int run_front(FstMlaCtx* c, int lid, const bf16* h_in) {
   prof_mark(c, FST_MLA_K_NORM_APPEND);
   NormAppendArgs na;
   na.cmp = c->d_cmp; na.q_norm = w.q_norm; na.kv_norm = w.kv_norm; na.lut = lut_of(c, lid);
-  na.dst_row = c->d_dst; na.qc = c->d_qc; na.kv_new = c->d_kvnew; na.pool = c->pools[lid];
+  na.dst_row = c->d_dst; na.qc = c->d_qc; na.kv_new = c->d_kvnew; na.pool = view_of(c, lid);
   na.T = T; na.q_lora = d.q_lora; na.kv_lora = d.kv_lora; na.row = d.row; na.rope = d.rope;
   na.eps = c->cfg.rms_eps;
   launch_norm_append(na, c->stream);
@@ -609,7 +624,7 @@ int run_back(FstMlaCtx* c, int lid, bf16* h_out) {
 // skip_single: the attention kernel finished the single-partial tokens; when every token with a
 // context is one, nothing is left to merge (tokens without any context still get their zero /
 // sink-only rows from the merge kernel).
-int run_merge_local(FstMlaCtx* c, int lid, int mode, float* rank_partial, bool skip_single = false) {
+int run_merge_local(FstMlaCtx* c, int lid, int mode, float* rank_partial, bool skip_single = false, bf16* o_lat = nullptr) {
   const Dims& d = c->d;
   const Sched& S = sched_of(c, lid);
   if (skip_single && S.min_tok_parts == 1 && S.max_tok_parts == 1) return FST_MLA_OK;
@@ -617,7 +632,7 @@ int run_merge_local(FstMlaCtx* c, int lid, int mode, float* rank_partial, bool s
   m.skip_single = skip_single ? 1 : 0;
   m.part_m = c->d_part_m; m.part_l = c->d_part_l; m.part_o = c->d_part_o; m.tok_part = S.d_tok_part;
   m.sinks = (d.v4 && mode == 0) ? c->layers[lid].sinks : nullptr;
-  m.lut = lut_of(c, lid); m.o_lat = c->d_olat; m.rank_partial = rank_partial;
+  m.lut = lut_of(c, lid); m.o_lat = o_lat ? o_lat : c->d_olat; m.rank_partial = rank_partial;
   m.T = c->T; m.H = d.H; m.d_v = d.d_v; m.rope = d.rope; m.inv_rope = inv_rope_heads(c, lid); m.mode = mode;
   // Up to six parts per token on average: a warp per row.  Twelve and more (a dozen tokens at most, as a
   // block or two per SM make partials): four blocks per row share the parts of a row (5 tokens x 27 parts,
@@ -700,6 +715,7 @@ int fst_cuda_mla_create(const FstMlaConfig* cfg, FstMlaCtx** out) {
   *out = x;  // from here on destroy() cleans up after a failure
 
   const size_t pool_elems = (size_t)c.n_pages * c.page_tokens * d.row;
+  x->page_bytes = (size_t)c.page_tokens * d.row * sizeof(bf16);
   const size_t T = c.max_tokens;
   int rc = FST_MLA_OK;
   for (int l = 0; l < c.n_layers && !rc; ++l) {
@@ -782,6 +798,10 @@ void fst_cuda_mla_destroy(FstMlaCtx* c) {
   }
   cudaFree(c->d_cproj);
   for (auto p : c->pools) cudaFree(p);
+  cudaFree(c->d_rows_tmp);
+  cudaFree(c->d_runs);
+  if (c->h_runs) cudaFreeHost(c->h_runs);
+  if (c->runs_ev) cudaEventDestroy(c->runs_ev);
   cudaFree(c->d_an);
   cudaFree(c->d_h); cudaFree(c->d_cmp); cudaFree(c->d_qc); cudaFree(c->d_kvnew); cudaFree(c->d_qfull);
   cudaFree(c->d_qeff); cudaFree(c->d_olat); cudaFree(c->d_low); cudaFree(c->d_out);
@@ -917,6 +937,7 @@ int fst_cuda_mla_set_layer_compressor(FstMlaCtx* c, int lid, const FstMlaCompres
   const int ratio = w ? w->ratio : 0;
   if (ratio != 0 && ratio != 4 && ratio != 128) return fail(FST_MLA_ERR_ARG, "compress ratio %d (0, 4 or 128)", ratio);
   if (ratio && (!w->wkv || !w->wgate || !w->ape || !w->norm)) return fail(FST_MLA_ERR_ARG, "a compressor tensor is NULL");
+  if (ratio && c->e4m3) return fail(FST_MLA_ERR_STATE, "the KV compressor writes bf16 rows: not with an E4M3 cache");
   for (int s = 0; s < c->cfg.max_seqs; ++s)
     if (c->live[s] && c->lens[s] > 0)
       return fail(FST_MLA_ERR_STATE, "set the compressors before any sequence holds rows");
@@ -1026,12 +1047,15 @@ int fst_cuda_mla_seq_truncate(FstMlaCtx* c, int32_t seq, int32_t n_tokens) {
   const int n_drop = c->lens[seq] - n_tokens;
   if (n_drop > 0) {
     std::vector<long long> offs(n_drop);
-    for (int i = 0; i < n_drop; ++i) offs[i] = row_offset(c, seq, n_tokens + i);
+    for (int i = 0; i < n_drop; ++i) offs[i] = c->e4m3 ? pool_row(c, seq, n_tokens + i) : row_offset(c, seq, n_tokens + i);
     long long* d_offs = nullptr;
     CU(cudaMalloc((void**)&d_offs, n_drop * sizeof(long long)));
     cudaError_t e = cudaMemcpyAsync(d_offs, offs.data(), n_drop * sizeof(long long), cudaMemcpyHostToDevice, c->stream);
     for (int l = 0; l < c->cfg.n_layers && e == cudaSuccess; ++l) {
-      launch_zero_rows(c->pools[l], d_offs, n_drop, c->d.row, c->stream);
+      if (c->e4m3)
+        launch_zero_rows_e4m3(view_of(c, l), d_offs, n_drop, c->stream);
+      else
+        launch_zero_rows(c->pools[l], d_offs, n_drop, c->d.row, c->stream);
       c->launches += 1;
     }
     if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
@@ -1115,7 +1139,7 @@ int fst_cuda_mla_reset(FstMlaCtx* c) {
     }
   std::fill(c->lens.begin(), c->lens.end(), 0);
   std::fill(c->live.begin(), c->live.end(), 0);
-  const size_t bytes = (size_t)c->cfg.n_pages * c->cfg.page_tokens * c->d.row * sizeof(bf16);
+  const size_t bytes = (size_t)c->cfg.n_pages * c->page_bytes;
   for (auto p : c->pools) CU(cudaMemsetAsync(p, 0, bytes, c->stream));
   CU(cudaStreamSynchronize(c->stream));
   c->planned = false;
@@ -1142,6 +1166,7 @@ int fst_cuda_mla_row_offset(FstMlaCtx* c, int32_t seq, int32_t pos, int64_t* off
   if (!seq_ok(c, seq)) return fail(FST_MLA_ERR_ARG, "sequence %d is not allocated", seq);
   if (pos < 0 || (size_t)pos >= c->tables[seq].size() * c->cfg.page_tokens)
     return fail(FST_MLA_ERR_ARG, "row %d has no page", pos);
+  if (c->e4m3) return fail(FST_MLA_ERR_STATE, "rows of an E4M3 cache lie in planes: no element offset (fst_cuda_mla_block_table names the page)");
   *off_out = row_offset(c, seq, pos);
   return FST_MLA_OK;
 }
@@ -1161,6 +1186,27 @@ static int cache_copy(FstMlaCtx* c, int lid, int32_t seq, int32_t pos0, int32_t 
   }
   const int pt = c->cfg.page_tokens, row = c->d.row;
   int done = 0;
+  if (c->e4m3) {
+    // through rows in device memory, quantised or turned back into bf16 on the device
+    while (done < n) {
+      RowRuns r;
+      int k = 0, turn = 0;
+      while (done + turn < n && turn < ROWS_TMP && k < RowRuns::CAP) {
+        const int pos = pos0 + done + turn, run = std::min({n - done - turn, pt - pos % pt, ROWS_TMP - turn});
+        r.run[k++] = RowRun{(int32_t)pool_row(c, seq, pos), turn, run};
+        turn += run;
+      }
+      uint16_t* host = rows + (size_t)done * row;
+      const size_t bytes = (size_t)turn * row * 2;
+      if (write) CU(cudaMemcpyAsync(c->d_rows_tmp, host, bytes, cudaMemcpyHostToDevice, c->stream));
+      CU(launch_rows_runs(view_of(c, lid), c->d_rows_tmp, r.run, nullptr, k, std::min(pt, turn), write, c->stream));
+      c->launches += 1;
+      if (!write) CU(cudaMemcpyAsync(host, c->d_rows_tmp, bytes, cudaMemcpyDeviceToHost, c->stream));
+      done += turn;
+    }
+    CU(cudaStreamSynchronize(c->stream));
+    return FST_MLA_OK;
+  }
   while (done < n) {  // one copy per page-contiguous run
     const int pos = pos0 + done, run = std::min(n - done, pt - pos % pt);
     bf16* dev = c->pools[lid] + row_offset(c, seq, pos);
@@ -1185,11 +1231,145 @@ int fst_cuda_mla_cache_read(FstMlaCtx* c, int lid, int32_t seq, int32_t pos0, in
 int fst_cuda_mla_pool_read(FstMlaCtx* c, int lid, uint16_t* out, size_t bytes) {
   if (!c || !out) return fail(FST_MLA_ERR_ARG, "null argument");
   if (lid < 0 || lid >= c->cfg.n_layers) return fail(FST_MLA_ERR_ARG, "layer %d out of range", lid);
-  const size_t full = (size_t)c->cfg.n_pages * c->cfg.page_tokens * c->d.row * 2;
+  const size_t full = (size_t)c->cfg.n_pages * c->page_bytes;
   if (bytes > full) return fail(FST_MLA_ERR_ARG, "pool holds %zu bytes", full);
   CU(cudaSetDevice(c->cfg.device));
   CU(cudaStreamSynchronize(c->stream));
   CU(cudaMemcpy(out, c->pools[lid], bytes, cudaMemcpyDeviceToHost));
+  return FST_MLA_OK;
+}
+
+int fst_cuda_mla_set_cache_format(FstMlaCtx* c, int32_t format) {
+  if (!c) return fail(FST_MLA_ERR_ARG, "null context");
+  if (format != FST_MLA_CACHE_BF16 && format != FST_MLA_CACHE_E4M3)
+    return fail(FST_MLA_ERR_ARG, "cache format %d (0: bf16, 1: E4M3)", format);
+  const bool e4m3 = format == FST_MLA_CACHE_E4M3;
+  if (e4m3 == c->e4m3) return FST_MLA_OK;
+  const Dims& d = c->d;
+  if (e4m3) {
+    if (d.rope % 8 || (d.row - d.rope) % 8 || d.row <= d.rope)
+      return fail(FST_MLA_ERR_ARG, "an E4M3 cache needs latent and rope widths that are multiples of 8");
+    if ((long long)c->cfg.n_pages * c->cfg.page_tokens >= (1ll << 31))
+      return fail(FST_MLA_ERR_ARG, "an E4M3 cache has fewer than 2^31 rows per layer");
+    if (c->has_cmp) return fail(FST_MLA_ERR_STATE, "the KV compressor writes bf16 rows: not with an E4M3 cache");
+  }
+  for (int s = 0; s < c->cfg.max_seqs; ++s)
+    if (c->live[s] && c->lens[s] > 0)
+      return fail(FST_MLA_ERR_STATE, "set the cache format before any sequence holds rows");
+  CU(cudaSetDevice(c->cfg.device));
+  CU(cudaStreamSynchronize(c->stream));
+  if (e4m3 && !c->d_rows_tmp) {
+    int rc = dev_alloc(&c->d_rows_tmp, (size_t)ROWS_TMP * d.row);
+    if (rc) return rc;
+  }
+  c->planned = false;
+  // layer by layer, so that the two forms of the cache are never held side by side; what fails leaves the
+  // old form behind (the memory for it has just been given back)
+  const size_t old_bytes = (size_t)c->cfg.n_pages * c->page_bytes;
+  const size_t new_page = (size_t)pool_view(nullptr, e4m3, d.row, d.rope, c->cfg.page_tokens).page_bytes;
+  const size_t new_bytes = (size_t)c->cfg.n_pages * new_page;
+  auto swap_pool = [&](int l, size_t bytes) {
+    cudaFree(c->pools[l]);
+    c->pools[l] = nullptr;
+    cudaError_t e = cudaMalloc((void**)&c->pools[l], bytes);
+    if (e == cudaSuccess) e = cudaMemset(c->pools[l], 0, bytes);
+    return e;
+  };
+  for (int l = 0; l < c->cfg.n_layers; ++l) {
+    cudaError_t e = swap_pool(l, new_bytes);
+    if (e == cudaSuccess) continue;
+    cudaGetLastError();
+    for (; l >= 0; --l) swap_pool(l, old_bytes);
+    return fail(FST_MLA_ERR_CUDA, "no memory for the cache in this format: %s", cudaGetErrorString(e));
+  }
+  c->e4m3 = e4m3;
+  c->page_bytes = new_page;
+  return FST_MLA_OK;
+}
+
+int fst_cuda_mla_cache_page_bytes(FstMlaCtx* c, int64_t* bytes_out) {
+  if (!c || !bytes_out) return fail(FST_MLA_ERR_ARG, "null argument");
+  *bytes_out = (int64_t)c->page_bytes;
+  return FST_MLA_OK;
+}
+
+int fst_cuda_mla_cache_append_device(FstMlaCtx* c, int lid, const void* d_rows) {
+  if (!c) return fail(FST_MLA_ERR_ARG, "null context");
+  if (lid < 0 || lid >= c->cfg.n_layers) return fail(FST_MLA_ERR_ARG, "layer %d out of range", lid);
+  if (!c->planned) return fail(FST_MLA_ERR_STATE, "no plan: call fst_cuda_mla_plan first");
+  if (c->T == 0) return FST_MLA_OK;
+  if (!d_rows || (reinterpret_cast<uintptr_t>(d_rows) & 15)) return fail(FST_MLA_ERR_ARG, "rows: null or not 16-byte aligned");
+  if (c->layers[lid].cmp_ratio)
+    return fail(FST_MLA_ERR_STATE, "layer %d has a KV compressor: its rows come with a layer call", lid);
+  CU(cudaSetDevice(c->cfg.device));
+  c->status_by_kernel = false;
+  CU(launch_rows_append(view_of(c, lid), (const bf16*)d_rows, c->d_dst, c->T, c->stream));
+  c->launches += 1;
+  return FST_MLA_OK;
+}
+
+int fst_cuda_mla_cache_read_device(FstMlaCtx* c, int lid, const FstMlaSeqStep* ranges, int32_t n_ranges, void* d_rows) {
+  if (!c || (!ranges && n_ranges > 0)) return fail(FST_MLA_ERR_ARG, "null argument");
+  if (lid < 0 || lid >= c->cfg.n_layers) return fail(FST_MLA_ERR_ARG, "layer %d out of range", lid);
+  if (n_ranges < 0) return fail(FST_MLA_ERR_ARG, "negative range count");
+  const int pt = c->cfg.page_tokens;
+  long long rows = 0, n_runs = 0;
+  int max_n = 0;
+  for (int b = 0; b < n_ranges; ++b) {
+    const FstMlaSeqStep& s = ranges[b];
+    if (!seq_ok(c, s.seq)) return fail(FST_MLA_ERR_ARG, "range %d: sequence %d is not allocated", b, s.seq);
+    if (s.pos0 < 0 || s.q_len < 0 || (long long)s.pos0 + s.q_len > c->lens[s.seq])
+      return fail(FST_MLA_ERR_ARG, "range %d: rows [%d, +%d) outside the sequence's %d", b, s.pos0, s.q_len, c->lens[s.seq]);
+    rows += s.q_len;
+    if (s.q_len > 0) n_runs += (s.pos0 + s.q_len - 1) / pt - s.pos0 / pt + 1;
+  }
+  if (rows == 0) return FST_MLA_OK;
+  if (rows >= (1ll << 31) || (long long)c->cfg.n_pages * pt >= (1ll << 31))
+    return fail(FST_MLA_ERR_CAPACITY, "at most 2^31 - 1 rows");
+  if (!d_rows || (reinterpret_cast<uintptr_t>(d_rows) & 15)) return fail(FST_MLA_ERR_ARG, "rows: null or not 16-byte aligned");
+  CU(cudaSetDevice(c->cfg.device));
+  // Few runs travel as an argument of the kernel.  More go through page-locked memory, which a captured
+  // copy would read at replay, when it holds another call's runs.
+  RowRun inl[RowRuns::CAP];
+  RowRun* out = inl;
+  const bool staged = n_runs > RowRuns::CAP;
+  if (staged) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    CU(cudaStreamIsCapturing(c->stream, &cap));
+    if (cap != cudaStreamCaptureStatusNone)
+      return fail(FST_MLA_ERR_STATE, "%lld pages in one read: capture at most %d", n_runs, RowRuns::CAP);
+    if (!c->runs_ev) CU(cudaEventCreateWithFlags(&c->runs_ev, cudaEventDisableTiming));
+    CU(cudaEventSynchronize(c->runs_ev));
+    if (n_runs > c->runs_cap) {
+      CU(cudaStreamSynchronize(c->stream));
+      if (c->h_runs) cudaFreeHost(c->h_runs);
+      cudaFree(c->d_runs);
+      c->h_runs = c->d_runs = nullptr;
+      c->runs_cap = 0;
+      const int cap_n = (int)std::max<long long>(4096, 2 * n_runs);
+      CU(cudaHostAlloc((void**)&c->h_runs, cap_n * sizeof(RowRun), cudaHostAllocDefault));
+      int rc = dev_alloc(&c->d_runs, (size_t)cap_n);
+      if (rc) return rc;
+      c->runs_cap = cap_n;
+    }
+    out = c->h_runs;
+  }
+  int k = 0, at = 0;
+  for (int b = 0; b < n_ranges; ++b)
+    for (int i = 0; i < ranges[b].q_len;) {
+      const int pos = ranges[b].pos0 + i, run = std::min(ranges[b].q_len - i, pt - pos % pt);
+      out[k++] = RowRun{(int32_t)pool_row(c, ranges[b].seq, pos), at, run};
+      max_n = std::max(max_n, run);
+      i += run;
+      at += run;
+    }
+  if (staged) {
+    CU(cudaMemcpyAsync(c->d_runs, c->h_runs, (size_t)k * sizeof(RowRun), cudaMemcpyHostToDevice, c->stream));
+    CU(cudaEventRecord(c->runs_ev, c->stream));
+  }
+  c->status_by_kernel = false;
+  CU(launch_rows_runs(view_of(c, lid), (bf16*)d_rows, inl, staged ? c->d_runs : nullptr, k, max_n, false, c->stream));
+  c->launches += 1;
   return FST_MLA_OK;
 }
 
@@ -1268,7 +1448,7 @@ int plan_tokens_part(FstMlaCtx* c, const FstMlaSeqStep* steps, int32_t n_seqs, i
       c->pl_tok_step[t] = b;
       for (int k = 0; k < 2; ++k)
         if (need[k]) memcpy(&c->pl_lut[k][(size_t)t * d.rope], lut_row_cached(c, k, rp0 + i), (size_t)d.rope * sizeof(float));
-      dst[t] = s.append ? row_offset(c, s.seq, s.pos0 + i) : -1;
+      dst[t] = !s.append ? -1 : c->e4m3 ? pool_row(c, s.seq, s.pos0 + i) : row_offset(c, s.seq, s.pos0 + i);
       tok_table[t] = toff;
       int len = s.append ? s.pos0 + s.q_len : s.pos0;
       if (causal && s.append) len = std::min(len, s.pos0 + i + 1);  // drop s > seq_pos_ + m (3626)
@@ -1566,7 +1746,7 @@ int plan_schedule_part(FstMlaCtx* c, bool on_copy_stream) {
     long long rows_once = 0;
     for (const FstMlaSeqStep& step : c->pl_steps)
       if (step.q_len > 0) rows_once += step.append ? step.pos0 + step.q_len : step.pos0;
-    S.tiles_in_l2 = S.by_blocks || (kv_rows >= 4 * rows_once && rows_once * c->d.row * (long long)sizeof(bf16) <= (64ll << 20));
+    S.tiles_in_l2 = S.by_blocks || (kv_rows >= 4 * rows_once && rows_once / c->cfg.page_tokens * (long long)c->page_bytes <= (64ll << 20));
     S.n_segs = S.n_parts = (int)segs.size();
     S.n_ctas = (int)cta_seg.size() - 1;
     S.kv_rows = kv_rows;
@@ -1789,7 +1969,7 @@ int fst_cuda_mla_append_rows(FstMlaCtx* c, int lid, const uint16_t* h_in, const 
   if ((rc = run_gemm(c, plain_gemm(rows, w.w_cmp, c->d_cmp, c->T, d.cmp_n, d.hidden)))) return rc;
   NormAppendArgs na;
   na.cmp = c->d_cmp; na.q_norm = w.q_norm; na.kv_norm = w.kv_norm; na.lut = lut_of(c, lid);
-  na.dst_row = c->d_dst; na.qc = c->d_qc; na.kv_new = c->d_kvnew; na.pool = c->pools[lid];
+  na.dst_row = c->d_dst; na.qc = c->d_qc; na.kv_new = c->d_kvnew; na.pool = view_of(c, lid);
   na.T = c->T; na.q_lora = d.q_lora; na.kv_lora = d.kv_lora; na.row = d.row; na.rope = d.rope;
   na.eps = c->cfg.rms_eps;
   launch_norm_append(na, c->stream);
@@ -1816,6 +1996,28 @@ int fst_cuda_mla_attention_only(FstMlaCtx* c, int lid, const uint16_t* q_eff, ui
   c->cur = nullptr;
   CU(cudaMemcpyAsync(o_lat, c->d_olat, (size_t)c->T * d.H * d.d_v * 2, cudaMemcpyDeviceToHost, c->stream));
   return fst_cuda_mla_sync(c);
+}
+
+int fst_cuda_mla_attention_device(FstMlaCtx* c, int lid, const void* d_q_eff, void* d_o_lat) {
+  if (!c) return fail(FST_MLA_ERR_ARG, "null context");
+  if (lid < 0 || lid >= c->cfg.n_layers) return fail(FST_MLA_ERR_ARG, "layer %d out of range", lid);
+  if (c->d.v4 && !c->layers[lid].set) return fail(FST_MLA_ERR_STATE, "layer %d has no weights (its sink logits)", lid);
+  if (!c->planned) return fail(FST_MLA_ERR_STATE, "no plan: call fst_cuda_mla_plan first");
+  if (c->T == 0) return FST_MLA_OK;
+  if (!d_q_eff || !d_o_lat || (reinterpret_cast<uintptr_t>(d_q_eff) & 15) || (reinterpret_cast<uintptr_t>(d_o_lat) & 15))
+    return fail(FST_MLA_ERR_ARG, "queries or output: null or not 16-byte aligned");
+  CU(cudaSetDevice(c->cfg.device));
+  int rc;
+  if ((rc = prof_begin(c))) return rc;
+  prof_mark(c, FST_MLA_K_ATTN);
+  bool direct = false;
+  if ((rc = run_attention(c, lid, (const bf16*)d_q_eff, &direct, (bf16*)d_o_lat))) return rc;
+  prof_mark(c, FST_MLA_K_MERGE);
+  if ((rc = run_merge_local(c, lid, 0, nullptr, direct, (bf16*)d_o_lat))) return rc;
+  prof_mark(c, FST_MLA_K_OPROJ_A);
+  c->cur = nullptr;
+  CU(cudaGetLastError());
+  return FST_MLA_OK;
 }
 
 int fst_cuda_mla_run_partial_device(FstMlaCtx* c, int lid, const void* d_h_in, void* d_partial) {

@@ -129,7 +129,7 @@ extern "C" int fst_cuda_mla_attention_noalloc(const void* d_q_eff, const void* d
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
   AttnArgs a;
   a.q_eff = static_cast<const bf16*>(d_q_eff);
-  a.pool = static_cast<const bf16*>(d_cache);
+  a.pool = pool_view(const_cast<void*>(d_cache), false, d_qk, 0, 64);
   a.tables = reinterpret_cast<const int32_t*>(sc + OFF_TABLE);
   a.segs = reinterpret_cast<const AttnSeg*>(sc + OFF_SEGS);
   a.cta_seg = nullptr;

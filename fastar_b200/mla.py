@@ -19,6 +19,7 @@ PRESET_BASELINE = 0
 PRESET_FASTAR_V4 = 1
 IMPL_AUTO, IMPL_TENSOR, IMPL_SIMT = 0, 1, 2
 STAGE_QC, STAGE_KV, STAGE_QEFF, STAGE_OLAT, STAGE_LOW, STAGE_OUT = range(6)
+CACHE_BF16, CACHE_E4M3 = 0, 1
 KERNEL_NAMES = ["compress", "norm_append", "q_expand", "q_absorb", "attn", "merge", "exchange", "merge_gathered",
                 "oproj_a", "oproj_b"]
 K_ATTN, K_MERGE = 4, 5
@@ -60,6 +61,18 @@ class CompressorW(C.Structure):
 class SeqStep(C.Structure):
     _fields_ = [("seq", C.c_int32), ("pos0", C.c_int32), ("q_len", C.c_int32),
                 ("rope_pos0", C.c_int32), ("append", C.c_int32), ("window", C.c_int32)]
+
+
+def seq_steps(steps):
+    """(seq, pos0, q_len[, rope_pos0[, append[, window]]]) tuples as the array the library takes (an array passes through:
+    a loop over the layers of a step converts them once)."""
+    if isinstance(steps, C.Array):
+        return steps
+    arr = (SeqStep * len(steps))()
+    for i, s in enumerate(steps):
+        s = tuple(s)
+        arr[i] = SeqStep(s[0], s[1], s[2], s[3] if len(s) > 3 else -1, s[4] if len(s) > 4 else 1, s[5] if len(s) > 5 else 0)
+    return arr
 
 
 def make_config(preset=PRESET_BASELINE, *, n_layers=1, n_pages=256, max_seqs=64, max_tokens=64, device=0,
@@ -104,6 +117,11 @@ def load_library() -> C.CDLL:
     L.fst_cuda_mla_cache_write.argtypes = [vp, C.c_int, i32, i32, i32, u16p]
     L.fst_cuda_mla_cache_read.argtypes = [vp, C.c_int, i32, i32, i32, u16p]
     L.fst_cuda_mla_pool_read.argtypes = [vp, C.c_int, u16p, C.c_size_t]
+    L.fst_cuda_mla_set_cache_format.argtypes = [vp, i32]
+    L.fst_cuda_mla_cache_page_bytes.argtypes = [vp, C.POINTER(i64)]
+    L.fst_cuda_mla_cache_append_device.argtypes = [vp, C.c_int, vp]
+    L.fst_cuda_mla_cache_read_device.argtypes = [vp, C.c_int, C.POINTER(SeqStep), i32, vp]
+    L.fst_cuda_mla_attention_device.argtypes = [vp, C.c_int, vp, vp]
     L.fst_cuda_mla_plan.argtypes = [vp, C.POINTER(SeqStep), i32, i32]
     L.fst_cuda_mla_run_device.argtypes = [vp, C.c_int, vp, vp]
     L.fst_cuda_mla_forward.argtypes = [vp, C.c_int, u16p, u16p, i32p, i32p, i32p, i32, i32]
@@ -340,7 +358,31 @@ class MlaContext:
         self._check(self.lib.fst_cuda_mla_cache_read(self._h, lid, seq, pos0, n, _u16(out)))
         return out
 
+    def set_cache_format(self, fmt: int) -> None:
+        """CACHE_BF16 or CACHE_E4M3 (8-bit latent values, groups of 64 with a power-of-two scale), before any
+        sequence holds rows."""
+        self._check(self.lib.fst_cuda_mla_set_cache_format(self._h, int(fmt)))
+
+    def cache_page_bytes(self) -> int:
+        n = C.c_int64()
+        self._check(self.lib.fst_cuda_mla_cache_page_bytes(self._h, C.byref(n)))
+        return n.value
+
+    def cache_append_device(self, lid: int, d_rows: int) -> None:
+        """Device rows bf16 [T, row] become the cache rows of the current plan's new tokens."""
+        self._check(self.lib.fst_cuda_mla_cache_append_device(self._h, lid, C.c_void_p(d_rows)))
+
+    def cache_read_device(self, lid: int, ranges, d_rows: int) -> None:
+        """ranges: (seq, pos0, n) tuples, or seq_steps() of them; their rows as bf16, one range behind the other."""
+        arr = seq_steps(ranges)
+        self._check(self.lib.fst_cuda_mla_cache_read_device(self._h, lid, arr, len(arr), C.c_void_p(d_rows)))
+
     def pool_read(self, lid: int) -> np.ndarray:
+        """A layer's pool as it is held: bf16 rows [n_pages * page_tokens, row], or (E4M3) bytes [n_pages, page bytes]."""
+        if self.cache_page_bytes() != self.cfg.page_tokens * self.dims["row"] * 2:
+            raw = np.empty((self.cfg.n_pages, self.cache_page_bytes()), np.uint8)
+            self._check(self.lib.fst_cuda_mla_pool_read(self._h, lid, raw.ctypes.data_as(C.POINTER(C.c_uint16)), raw.nbytes))
+            return raw
         out = np.empty((self.cfg.n_pages * self.cfg.page_tokens, self.dims["row"]), np.uint16)
         self._check(self.lib.fst_cuda_mla_pool_read(self._h, lid, _u16(out), out.nbytes))
         return out
@@ -348,11 +390,7 @@ class MlaContext:
     # -- the layer --
     def plan(self, steps, causal: bool = False) -> int:
         """steps: iterable of (seq, pos0, q_len[, rope_pos0[, append[, window]]]).  Returns T."""
-        arr = (SeqStep * len(steps))()
-        for i, s in enumerate(steps):
-            s = tuple(s)
-            arr[i] = SeqStep(s[0], s[1], s[2], s[3] if len(s) > 3 else -1, s[4] if len(s) > 4 else 1,
-                             s[5] if len(s) > 5 else 0)
+        arr = seq_steps(steps)
         self._check(self.lib.fst_cuda_mla_plan(self._h, arr, len(steps), int(causal)))
         return self.plan_tokens()
 
@@ -418,11 +456,7 @@ class MlaContext:
         """The split-KV layer call with host buffers; steps as for plan()."""
         h = np.ascontiguousarray(h, np.uint16)
         out = np.empty_like(h)
-        arr = (SeqStep * len(steps))()
-        for i, s in enumerate(steps):
-            s = tuple(s)
-            arr[i] = SeqStep(s[0], s[1], s[2], s[3] if len(s) > 3 else -1, s[4] if len(s) > 4 else 1,
-                             s[5] if len(s) > 5 else 0)
+        arr = seq_steps(steps)
         self._check(self.lib.fst_cuda_mla_forward_split(self._h, lid, _u16(h), _u16(out), arr, len(steps), int(causal)))
         return out
 
@@ -462,6 +496,10 @@ class MlaContext:
         out = np.empty((T * self.cfg.n_heads, self.dims["d_v"]), np.uint16)
         self._check(self.lib.fst_cuda_mla_attention_only(self._h, lid, _u16(q_eff), _u16(out)))
         return out
+
+    def attention_device(self, lid: int, d_q_eff: int, d_o_lat: int) -> None:
+        """attention_only() on device buffers: bf16 [T * heads, d_qk] -> bf16 [T * heads, d_v]."""
+        self._check(self.lib.fst_cuda_mla_attention_device(self._h, lid, C.c_void_p(d_q_eff), C.c_void_p(d_o_lat)))
 
     def get_stage(self, stage: int) -> np.ndarray:
         T, H, d, c = self.plan_tokens(), self.cfg.n_heads, self.dims, self.cfg

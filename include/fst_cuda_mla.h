@@ -44,6 +44,10 @@ extern "C" {
 #define FST_MLA_IMPL_TENSOR 1 /* tcgen05 / TMEM / TMA kernels */
 #define FST_MLA_IMPL_SIMT 2   /* CUDA-core kernels (any shape) */
 
+/* What the cache pages hold (fst_cuda_mla_set_cache_format). */
+#define FST_MLA_CACHE_BF16 0
+#define FST_MLA_CACHE_E4M3 1
+
 typedef struct FstMlaCtx FstMlaCtx;
 
 /* Shape constants mirror include/fst_engine.h:92-95 (MLA_Q_LORA, MLA_KV_LORA, MLA_N_HEADS,
@@ -224,7 +228,32 @@ int fst_cuda_mla_cache_write(FstMlaCtx* ctx, int lid, int32_t seq, int32_t pos0,
                              const uint16_t* rows);
 int fst_cuda_mla_cache_read(FstMlaCtx* ctx, int lid, int32_t seq, int32_t pos0, int32_t n,
                             uint16_t* rows);
-/* Raw pool of a layer [n_pages * page_tokens, row] to host. */
+/* What the pages hold from here on; set before any sequence holds rows (the pools are laid out anew,
+ * all zeros).  FST_MLA_CACHE_E4M3: the latent values of a row in 8 bits, in groups of 64 with a power-of-two
+ * scale of their own, the rope dims in bf16: 648 bytes per 576-wide row instead of 1152, 584 per 512-wide
+ * row instead of 1024.  A group x: k is the least integer with max |x| <= 448 * 2^k, kept within
+ * [-100, 120]; a value is held as x * 2^-k rounded to E4M3 (nearest even) and stands for that times 2^k,
+ * which is a bf16 value.  Magnitudes above 1.875 * 2^127, infinities among them, saturate there; a NaN makes its
+ * whole group NaN.  Every call that writes rows quantises them (the layer calls, append_rows, cache_write,
+ * cache_append_device), every call that reads them gives the bf16 values they stand for (cache_read,
+ * cache_read_device), and the attention multiplies exactly these values.  A layer call's own new rows are
+ * attended to in their quantised form.  Not with a KV compressor (its rows are bf16), and
+ * fst_cuda_mla_row_offset has no answer then.  FST_MLA_ERR_STATE if a sequence holds rows or a layer has
+ * a compressor, FST_MLA_ERR_ARG if latent or rope width is no multiple of 8. */
+int fst_cuda_mla_set_cache_format(FstMlaCtx* ctx, int32_t format);
+/* Bytes of a page of page_tokens rows in one layer's pool, in the present format. */
+int fst_cuda_mla_cache_page_bytes(FstMlaCtx* ctx, int64_t* bytes_out);
+/* Given rows enter the cache, for hosts that make them themselves: row t of d_rows (device bf16 [T, row], 16-byte
+ * aligned, normed and rotated) becomes the cache row of new token t of the current plan; tokens of steps with
+ * append = 0 have none.  What cache_write does for host rows, without its copies.  Enqueued on the context's
+ * stream, no synchronisation; may be captured into a graph (valid until the next plan). */
+int fst_cuda_mla_cache_append_device(FstMlaCtx* ctx, int lid, const void* d_rows);
+/* Cached rows back as bf16: of every range, rows pos0 .. pos0 + q_len - 1 of sequence seq (the other members
+ * are not read; the same sequence may appear more than once), one range behind the other, to d_rows (device bf16
+ * [sum q_len, row], 16-byte aligned).  Needs no plan.  Enqueued on the context's stream, no synchronisation; a
+ * call that spans up to 250 pages may be captured into a graph, a longer one returns FST_MLA_ERR_STATE there. */
+int fst_cuda_mla_cache_read_device(FstMlaCtx* ctx, int lid, const FstMlaSeqStep* ranges, int32_t n_ranges, void* d_rows);
+/* Raw pool of a layer to host: [n_pages * page_tokens, row] bf16, or the pages of an E4M3 cache. */
 int fst_cuda_mla_pool_read(FstMlaCtx* ctx, int lid, uint16_t* out, size_t bytes);
 
 /* ---- the layer ------------------------------------------------------------------------ */
@@ -272,6 +301,10 @@ int fst_cuda_mla_forward(FstMlaCtx* ctx, int lid, const uint16_t* h_in, uint16_t
  * src/fst_engine.cpp:3588, 3682): host q_eff [T*H, d_qk] -> host o_lat [T*H, d_v], over the
  * cache as it stands, for the current plan (nothing is appended). */
 int fst_cuda_mla_attention_only(FstMlaCtx* ctx, int lid, const uint16_t* q_eff, uint16_t* o_lat);
+/* The same with device buffers: d_q_eff bf16 [T*H, d_qk] -> d_o_lat bf16 [T*H, d_v], both 16-byte aligned (not
+ * the same buffer).  Enqueued on the context's stream, no synchronisation; may be captured into a graph, which
+ * is valid until the next plan.  Layer weights are needed in the V4 form only (the sink logits). */
+int fst_cuda_mla_attention_device(FstMlaCtx* ctx, int lid, const void* d_q_eff, void* d_o_lat);
 /* Split-KV across GPUs: run the layer up to the merged per-GPU partial.  d_partial is device
  * fp32 [T*H, 2 + d_v] holding (max, sum, un-normalised O) per query row. */
 int fst_cuda_mla_run_partial_device(FstMlaCtx* ctx, int lid, const void* d_h_in, void* d_partial);

@@ -29,6 +29,8 @@
 //   lanes 16-31: O[64, 512] in columns [0,512)  (its MMAs take A = P from shared memory)
 // The softmax threads touch lanes 0-15 only through the 16-lane access shape (O is rescaled the
 // same way at lane offset 16); 32-lane loads are used where the other 16 lanes are only read.
+#include <type_traits>
+
 #include "kernels.cuh"
 #include "tc_common.cuh"
 
@@ -42,7 +44,8 @@ constexpr int D_V = 512;
 constexpr int CHUNK = TILE * 128;      // 8 KB: [64 tok x 64 dims]
 constexpr int P_BYTES = HEADS * TILE * 2;  // 8 KB
 constexpr int ST_THREADS = 448;  // warps: 0, 10, 11 copy; 1, 13 issue QK; 12 issues SV; 2-9 softmax
-constexpr int E8_THREADS = 512;  // E4M3 cache: 0 copies; 1, 10 issue QK (1: the Q_eff copies too); 11 issues SV; 12-15 dequantise
+constexpr int E8_THREADS = 640;  // E4M3 cache: 0 copies; 1, 10 issue QK (1: the Q_eff copies too); 11 issues SV; 12-19 dequantise
+constexpr int E8_DEQ_WARPS = 8;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t COL_Q = 0, COL_S = 288, COL_O = 0;
 constexpr uint32_t LANE16 = 16u << 16;
@@ -301,6 +304,21 @@ __device__ __forceinline__ void bulk_load_hint(void* dst, const void* src, uint3
                : "memory");
 }
 
+// 16 bytes of shared memory by 32-bit address (the kernel's base pointer is aligned by integer arithmetic, behind
+// which the compiler no longer knows it for shared memory).
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
 // A barrier wait of a whole warp: all lanes go on, or none.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* d_status, int code) {
   return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_flag, d_status, code));
@@ -347,7 +365,14 @@ __device__ __forceinline__ bool qk_chunks(StreamMisc* mi, int g, uint32_t d, uin
 // waiting for it to free a buffer -- the better trade when tiles come from L2 (blocks of query
 // tokens: the kernel is bound by its own pipeline there; attention of the 32 x 16 x 16384 verify block
 // 1.69 -> 1.55 ms), the worse one when the life of a frame bounds the kernel (decode: 86 -> 88 us).
-// E8: the cache is held in E4M3 (cache_rows.cuh).
+// E8: the cache is held in E4M3 (cache_rows.cuh).  What bounds it: the life of a frame, two frames per SM.  From the
+// moment the SV MMAs of a frame's tile retire it takes 300 cycles until the dequantising warps know, 1100 to
+// store the next tile (72 KB, from registers), 2000 for its QK MMAs (which share the tensor pipe with the
+// other tile's SV), 1400 for the softmax and 1600 for the SV MMAs; a tile every 3500 cycles, of which the pipe is
+// busy 2176 and HBM would need 1600.  With the dequantisation behind the wait for the frame instead of in front
+// of it the same tile took 4300 (64 users x 1024-8192 rows 94 us, now 82), by four warps instead of eight 4850
+// (117), with a branch on the scale per 16 codes 7000 (133).  Chunks 0-3 released after the first half of the SV
+// MMAs: 88.
 template <int NCH, bool DIRECT, bool WHOLE, bool FLAT, bool E8>
 __global__ void __launch_bounds__(E8 ? E8_THREADS : ST_THREADS, 1)
 k_attn_stream(const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ CUtensorMap tmQ, StreamParams p) {
@@ -365,7 +390,7 @@ k_attn_stream(const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ 
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 4; ++i) {
-      for (int j = 0; j < 3; ++j) tc::mbar_init(&mi->full_t[i][j], E8 ? 4 : j < 2 ? 3 : NCH - 6);
+      for (int j = 0; j < 3; ++j) tc::mbar_init(&mi->full_t[i][j], E8 ? E8_DEQ_WARPS : j < 2 ? 3 : NCH - 6);
       tc::mbar_init(&mi->o_done[i], 1);
     }
     tc::mbar_init(&mi->q_ready, 256);
@@ -376,7 +401,7 @@ k_attn_stream(const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ 
       for (int i = 0; i < 2; ++i) {
         tc::mbar_init(&mi->st_full[i][0], 1);
         tc::mbar_init(&mi->st_full[i][1], 1);
-        tc::mbar_init(&mi->st_free[i], 4);
+        tc::mbar_init(&mi->st_free[i], E8_DEQ_WARPS);
       }
     mi->abort_flag = 0;
     tc::fence_barrier_init();
@@ -472,9 +497,9 @@ k_attn_stream(const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ 
             const uint64_t policy = tc::l2_policy_evict_normal();
 #pragma unroll
             for (int i = 0; i < 3; ++i) {
-              uint64_t* bar = &mi->full_t[gq & 3][i];  // four arrivals, as the dequantising warps make of a tile's
+              uint64_t* bar = &mi->full_t[gq & 3][i];  // as many arrivals as the dequantising warps make for a tile
               tc::mbar_expect_tx(bar, (i < 2 ? 3 : NCH - 6) * CHUNK);
-              for (int a = 0; a < 3; ++a) tc::mbar_arrive(bar);
+              for (int a = 1; a < E8_DEQ_WARPS; ++a) tc::mbar_arrive(bar);
 #pragma unroll
               for (int c = 3 * i; c < 3 * i + 3 && c < NCH; ++c)
                 tc::tma_load_3d_hint(s_ring + ((gq % F) * NCH + c) * CHUNK, &tmQ, bar, c * 64, cur.sg.tok * HEADS, 0, policy);
@@ -536,53 +561,115 @@ k_attn_stream(const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ 
         cur.next(p);
       }
     }
-  } else if (warp >= 12) {
-    // ---------------- E8: stages -> frames (warps 12-15, one on each scheduler) ----------------
-    // A thread has a quarter (16 codes) of two tokens' rows in every group.  Reads of a warp are 512 contiguous bytes;
+  } else if (E8 && warp >= 12) {
+    // ---------------- E8: stages -> frames (warps 12-19, two on each scheduler) ----------------
+    // A thread has a quarter (16 codes) of one token's row in every group.  Reads of a warp are 512 contiguous bytes;
     // its stores of 16 bytes meet eight different units of the 128-byte swizzle per eight lanes: no bank is
     // met twice in either.
     if constexpr (E8) {
       const int ct = threadIdx.x - 12 * 32, tk = ct >> 2, qd = ct & 3;
+      const uint32_t smem0 = tc::smem_u32(smem);
+      const uint32_t u0 = ((2 * qd) ^ (tk & 7)) * 16, u1 = ((2 * qd + 1) ^ (tk & 7)) * 16;
+      bool ready = false;  // the first piece of the current tile's page is known to be there
       while (!cur.done()) {
         const int g = cur.g, n = cur.n;
+        const uint32_t par = (n >> 1) & 1;
+        if (!__all_sync(0xffffffffu, ready) &&
+            !warp_wait(&mi->st_full[n & 1][0], par, abort_flag, p.d_status, ST_DEQ_TIMEOUT)) break;
+        const uint32_t stage = smem0 + off_stage(NCH, E8) + (n & 1) * e8_page(NCH), frame = smem0 + (g % F) * (NCH * CHUNK);
+        const uint32_t codes = stage + E8_CODES_OFF + tk * 64 + qd * 16, out = frame + tk * 128;
+        const uint2 sb = lds64(stage + tk * 8);
+        // scales that are no normal fp16 numbers (beyond 2^-14 .. 2^15) and NaN marks, decided once per tile; bytes of 0
+        // (slots without a row, groups of zeros) go with any factor
+        const uint32_t d1 = 0x01010101u, lo = 0x70707070u, hi = 0x8E8E8E8Eu;
+        const bool wide = __any_sync(0xffffffffu, (__vcmpgtu4(sb.x, hi) | __vcmpgtu4(sb.y, hi) | __vcmpltu4(__vsub4(sb.x, d1), lo) |
+                                                   __vcmpltu4(__vsub4(sb.y, d1), lo)) != 0);
+        auto scale_byte = [&](int c) { return ((c < 4 ? sb.x : sb.y) >> (8 * (c & 3))) & 255u; };
+        auto store = [&](int c, const uint2* o) {
+          sts128(out + c * CHUNK + u0, o[0].x, o[0].y, o[1].x, o[1].y);
+          sts128(out + c * CHUNK + u1, o[2].x, o[2].y, o[3].x, o[3].y);
+        };
+        // the rope dims as they are, in the swizzle of the other chunks
+        auto store_rope = [&](int i, uint4 v) {
+          const int t = (ct >> 3) + 32 * i, u = ct & 7;
+          sts128(frame + (NCH - 1) * CHUNK + t * 128 + ((u ^ (t & 7)) * 16), v.x, v.y, v.z, v.w);
+        };
+        auto load_rope = [&](int i) { return lds128(stage + E8_SCALES + ct * 16 + i * (32 * 128)); };
         // the frame is free once the SV MMAs of the slot F back have retired
-        if (g >= F && !warp_wait(&mi->o_done[(g - F) & 3], ((g - F) >> 2) & 1, abort_flag, p.d_status, ST_DEQ_TIMEOUT)) break;
-        if (!warp_wait(&mi->st_full[n & 1][0], (n >> 1) & 1, abort_flag, p.d_status, ST_DEQ_TIMEOUT)) break;
-        const unsigned char* stage = smem + off_stage(NCH, E8) + (n & 1) * e8_page(NCH);
-        unsigned char* frame = s_ring + (g % F) * (NCH * CHUNK);
-        const uint2 sb[2] = {*reinterpret_cast<const uint2*>(stage + tk * 8), *reinterpret_cast<const uint2*>(stage + (tk + 32) * 8)};
-        bool ok = true;
-#pragma unroll 1
-        for (int c = 0; c < NCH - 1; ++c) {
-          if (c == 3) ok = warp_wait(&mi->st_full[n & 1][1], (n >> 1) & 1, abort_flag, p.d_status, ST_DEQ_TIMEOUT);
-          if (!ok) break;
+        auto frame_free = [&]() {
+          return g < F || warp_wait(&mi->o_done[(g - F) & 3], ((g - F) >> 2) & 1, abort_flag, p.d_status, ST_DEQ_TIMEOUT);
+        };
+        auto arrive = [&](int i) {
+          tc::fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&mi->full_t[g & 3][i]);
+        };
+        auto stage_read = [&]() {
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&mi->st_free[n & 1]);
+        };
+        auto second_piece = [&]() { return warp_wait(&mi->st_full[n & 1][1], par, abort_flag, p.d_status, ST_DEQ_TIMEOUT); };
+        if (!wide) {
+          // The whole tile is turned in registers (72 per thread) while its frame is still being read: the registers of
+          // these warps are a third frame.  What is left once the frame is free is stores, and the stage is free
+          // for the page after next before that.
+          uint2 o[8][4];
+          uint4 rp[2] = {load_rope(0), load_rope(1)};
+          auto turn = [&](int c, uint4 w4) {
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int t = tk + 32 * i;
-            const uint4 w4 = *reinterpret_cast<const uint4*>(stage + E8_CODES_OFF + c * E8_GROUP + t * 64 + qd * 16);
+            for (int k = 0; k < 4; ++k) o[c][k] = e4m3_to_bf16x4_near(w[k], (uint32_t)(scale_byte(c) - 112) << 10);
+          };
+          {
+            const uint4 w0 = lds128(codes), w1 = lds128(codes + E8_GROUP), w2 = lds128(codes + 2 * E8_GROUP);
+            turn(0, w0);
+            turn(1, w1);
+            turn(2, w2);
+          }
+          if (!second_piece()) break;
+          {
+            const uint4 w3 = lds128(codes + 3 * E8_GROUP), w4 = lds128(codes + 4 * E8_GROUP), w5 = lds128(codes + 5 * E8_GROUP);
+            turn(3, w3);
+            turn(4, w4);
+            turn(5, w5);
+          }
+          {
+            const uint4 w6 = lds128(codes + 6 * E8_GROUP);
+            uint4 w7 = w6;
+            if (NCH == 9) w7 = lds128(codes + 7 * E8_GROUP);
+            turn(6, w6);
+            if (NCH == 9) turn(7, w7);
+          }
+          stage_read();
+          if (!frame_free()) break;
+#pragma unroll
+          for (int c = 0; c < 3; ++c) store(c, o[c]);
+          arrive(0);
+#pragma unroll
+          for (int c = 3; c < 6; ++c) store(c, o[c]);
+          arrive(1);
+#pragma unroll
+          for (int c = 6; c < NCH - 1; ++c) store(c, o[c]);
+          store_rope(0, rp[0]);
+          store_rope(1, rp[1]);
+        } else {
+          if (!second_piece() || !frame_free()) break;
+#pragma unroll 1
+          for (int c = 0; c < NCH - 1; ++c) {
+            const uint4 w4 = lds128(codes + c * E8_GROUP);
             const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
             uint2 o[4];
-            e4m3_dequant<4>(w, ((c < 4 ? sb[i].x : sb[i].y) >> (8 * (c & 3))) & 255u, o);
-            unsigned char* dst = frame + c * CHUNK + t * 128;
-            *reinterpret_cast<uint4*>(dst + (((2 * qd) ^ (t & 7)) * 16)) = make_uint4(o[0].x, o[0].y, o[1].x, o[1].y);
-            *reinterpret_cast<uint4*>(dst + (((2 * qd + 1) ^ (t & 7)) * 16)) = make_uint4(o[2].x, o[2].y, o[3].x, o[3].y);
+            e4m3_dequant<4>(w, scale_byte(c), o);
+            store(c, o);
+            if (c == 2 || c == 5) arrive(c / 3);
           }
-          if (c == NCH - 2) {  // the rope dims as they are, in the swizzle of the other chunks
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int t = (ct >> 3) + 16 * i, u = ct & 7;
-              *reinterpret_cast<uint4*>(frame + (NCH - 1) * CHUNK + t * 128 + ((u ^ (t & 7)) * 16)) =
-                  *reinterpret_cast<const uint4*>(stage + E8_SCALES + t * 128 + u * 16);
-            }
-          }
-          if (c == 2 || c == 5 || c == NCH - 2) {
-            tc::fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&mi->full_t[g & 3][c == 2 ? 0 : c == 5 ? 1 : 2]);
-          }
+          store_rope(0, load_rope(0));
+          store_rope(1, load_rope(1));
+          stage_read();
         }
-        if (!ok) break;
-        if (lane == 0) tc::mbar_arrive(&mi->st_free[n & 1]);  // (behind the last __syncwarp: the stage has been read)
+        // the next page is asked for before this tile's last arrival: the answer takes a few hundred cycles
+        ready = tc::mbar_test_wait(&mi->st_full[(n + 1) & 1][0], ((n + 1) >> 1) & 1);
+        arrive(2);
         cur.next(p);
       }
     }
@@ -826,6 +913,8 @@ cudaError_t launch_attn_stream(const AttnArgs& a, cudaStream_t st) {
          : p.direct ? FST_ATTN_LAUNCH(NCHV, true, false, false, E8V) : FST_ATTN_LAUNCH(NCHV, false, false, false, E8V))
   if (a.flat_rows > 0)
     return a.d_qk == 576 ? FST_ATTN_LAUNCH(9, false, false, true, false) : FST_ATTN_LAUNCH(8, false, false, true, false);
+  // E4M3 takes the bf16 kernel's rule: scores are then added in the same order, and the output has the bits that a bf16
+  // cache of the same values gives (whole tiles always: 64 users 81.9 us against 83.0)
   if (a.pool.e4m3) return a.d_qk == 576 ? FST_ATTN_PICK(9, true) : FST_ATTN_PICK(8, true);
   return a.d_qk == 576 ? FST_ATTN_PICK(9, false) : FST_ATTN_PICK(8, false);
 #undef FST_ATTN_PICK

@@ -3,7 +3,8 @@
 // bf16: rows one behind the other, row r of the pool at r * row elements.
 //
 // E4M3: a page of pt rows is one block of three planes,
-//   scales [pt, sp] bytes   one E8M0 byte per group of 64 latent values: 2^(b - 127); 255: the group holds a NaN
+//   scales [pt, sp] bytes   one E8M0 byte per group of 64 latent values: 2^(b - 127); 255: the group holds a NaN; 0:
+//                           all its values are 0, as in a slot that holds no row
 //   rope   [pt, rope] bf16  the rotated dims as they are (they carry the position and are few)
 //   codes  [groups][pt, 64] E4M3 values, group by group: a group of a page (4 KB) is one contiguous
 //                           block, the source of one 64-column chunk of the attention's tile
@@ -67,6 +68,7 @@ __device__ __forceinline__ long long e4m3_code_off(const PoolView& v, int s, int
 // larger than every number's).
 __device__ __forceinline__ int e4m3_scale_byte(uint32_t amax_bits) {
   if (amax_bits > 0x7F800000u) return 255;
+  if (amax_bits == 0) return 0;  // what slots without a row have
   amax_bits = min(amax_bits, 0x7F700000u);  // 1.875 * 2^127
   // a = m * 2^e with 1 <= m < 2; 448 = 1.75 * 2^8
   const int k = (int)(amax_bits >> 23) - 127 - 8 + ((amax_bits & 0x7FFFFFu) > 0x600000u);
@@ -101,6 +103,28 @@ __device__ __forceinline__ uint2 e4m3_to_bf16x4(uint32_t w, __nv_bfloat162 mult)
 __device__ __forceinline__ __nv_bfloat162 bf162_of_bits(uint32_t bits16) {
   const uint32_t w = bits16 | (bits16 << 16);
   return *reinterpret_cast<const __nv_bfloat162*>(&w);
+}
+// The same where 2^k is a normal fp16 number (scale bytes 113 .. 142): codes to fp16, a multiplication that widens to
+// fp32, two packed to bf16; every step exact.  On the integer pipe a pair of codes costs half of what the
+// bit moves above do (16 x 2048 codes per warp of four: 1630 cycles instead of 2110, loads and stores included).
+// scale_f16: the bits of 2^k.
+__device__ __forceinline__ uint2 e4m3_to_bf16x4_near(uint32_t w, uint32_t scale_f16) {
+  float f0, f1, f2, f3;
+  asm("{\n\t.reg .b16 a, b, s, z0, z1, z2, z3;\n\t.reg .b32 h0, h1;\n\t"
+      "mov.b32 {a, b}, %4;\n\t"
+      "mov.b32 {s, z0}, %5;\n\t"
+      "cvt.rn.f16x2.e4m3x2 h0, a;\n\t"
+      "cvt.rn.f16x2.e4m3x2 h1, b;\n\t"
+      "mov.b32 {z0, z1}, h0;\n\t"
+      "mov.b32 {z2, z3}, h1;\n\t"
+      "fma.rn.f32.f16 %0, z0, s, %6;\n\t"
+      "fma.rn.f32.f16 %1, z1, s, %6;\n\t"
+      "fma.rn.f32.f16 %2, z2, s, %6;\n\t"
+      "fma.rn.f32.f16 %3, z3, s, %6;\n\t}"
+      : "=f"(f0), "=f"(f1), "=f"(f2), "=f"(f3)
+      : "r"(w), "r"(scale_f16), "f"(-0.0f));  // (-0: a code of -0 stays -0)
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(f0, f1), hi = __floats2bfloat162_rn(f2, f3);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
 }
 // N words of four codes each, under the scale byte b.
 template <int N>

@@ -324,6 +324,38 @@ def test_attention_over_quantised_rows(torch, preset, batch, causal, impl):
                         64, v4)
 
 
+@pytest.mark.parametrize("factor", [2.0 ** -40, 2.0 ** 20, 0.0, math.nan])
+@pytest.mark.parametrize("preset", [mla.PRESET_BASELINE, mla.PRESET_FASTAR_V4])
+def test_scales_of_every_size(torch, preset, factor):
+    """Groups whose scale is no fp16 number, groups of zeros and of NaN among ordinary ones: what a bf16 cache of the
+    same values gives, bit for bit."""
+    rng = np.random.default_rng(13)
+    with make(preset, n_pages=40) as ctx, make(preset, e4m3=False, n_pages=40) as plain:
+        row = ctx.dims["row"]
+        w = {n: np.zeros(sh, np.uint16) for n, sh in mla.weight_shapes(ctx.cfg).items()}
+        w["attn_sinks"] = np.zeros(64, np.float32)
+        x = rng.standard_normal((400, row)).astype(np.float32) * np.float32(2.0 ** -12)
+        x[130, 64:128] *= np.float32(factor)   # one group of one row of the third page
+        x[300:320, :448] *= np.float32(factor)
+        q = bits(rng.standard_normal((2 * 64, row)).astype(np.float32))
+        outs = []
+        for c in (ctx, plain):
+            c.set_layer_weights(0, w)
+            s, t = c.seq_alloc(), c.seq_alloc()
+            c.cache_write(0, s, 0, bits(x) if c is ctx else values)
+            c.cache_write(0, t, 0, bits(x[:130]))
+            values = c.cache_read(0, s, 0, 400)
+            if c is plain:
+                c.cache_write(0, t, 0, ctx.cache_read(0, t, 0, 130))
+            c.plan([(s, 400, 1, -1, 0), (t, 130, 1, -1, 0)])
+            o = dev(torch, np.zeros((2 * 64, 512), np.uint16))
+            c.attention_device(0, dev(torch, q).data_ptr(), o.data_ptr())
+            c.sync()
+            outs.append(f32(host(o)))
+        assert np.array_equal(outs[0], outs[1], equal_nan=True)
+        assert np.isfinite(outs[0][64:]).all() and np.isnan(outs[0][:64]).any() == math.isnan(factor)
+
+
 def test_attention_without_rows(torch):
     """Tokens that see nothing get zeros, also beside tokens that see something."""
     with make() as ctx:

@@ -60,6 +60,21 @@ __global__ void __launch_bounds__(ROW_WARPS * 32) k_rows_runs(PoolView v, bf16* 
   }
 }
 
+// E4M3 pages pages[i] -> page i of a bf16 pool: eight blocks per page, a thread one or two units of eight values at a
+// time.  Bound by bytes: 41 KB in and 74 KB out per page of 64 576-wide rows.
+__global__ void __launch_bounds__(256) k_pages_expand(PoolView v, const int32_t* pages, bf16* out) {
+  pdl_launch();
+  const int page = pages[blockIdx.y];  // (the plan's, not an earlier kernel's)
+  pdl_wait();
+  const int units = v.row / 8, n = v.pt * units;
+  const long long r0 = (long long)page * v.pt;
+  uint4* dst = reinterpret_cast<uint4*>(out + (long long)blockIdx.y * v.pt * v.row);
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) {
+    const int s = i / units;
+    dst[i] = load_unit(v, r0 + s, i - s * units);
+  }
+}
+
 // Slots [0, keep) of page `src` -> page `dst`, zeros behind them.  Bits are moved as they are held.
 // (Zeros, not what the source has there: a masked row is multiplied by a probability of 0.)
 __global__ void __launch_bounds__(256) k_page_copy(PoolView v, int src, int dst, int keep) {
@@ -120,6 +135,10 @@ cudaError_t launch_rows_runs(const PoolView& v, bf16* buf, const RowRun* host_ru
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
+}
+
+cudaError_t launch_expand_pages(const PoolView& v, const int32_t* pages, int n, bf16* out, cudaStream_t st) {
+  return launch_pdl(k_pages_expand, dim3(8, n), dim3(256), 0, st, 1, v, pages, out);
 }
 
 cudaError_t launch_page_copy(const PoolView& v, int src, int dst, int keep, cudaStream_t st) {

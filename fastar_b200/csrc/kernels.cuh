@@ -274,6 +274,8 @@ struct RowRuns {  // runs that travel as a kernel argument
 // host_runs (at most RowRuns::CAP, passed by value) or dev_runs; max_n: rows of the longest run.
 cudaError_t launch_rows_runs(const PoolView& v, bf16* buf, const RowRun* host_runs, const RowRun* dev_runs, int n_runs, int max_n,
                              bool write, cudaStream_t st);
+// E4M3 pages -> bf16 pages 0 .. n-1 of `out`.
+cudaError_t launch_expand_pages(const PoolView& v, const int32_t* pages, int n, bf16* out, cudaStream_t st);
 cudaError_t launch_page_copy(const PoolView& v, int src, int dst, int keep, cudaStream_t st);
 void launch_zero_rows_e4m3(const PoolView& v, const long long* rows, int n_rows, cudaStream_t st);
 

@@ -88,6 +88,11 @@ struct Sched {
   int max_tok_parts = 0, min_tok_parts = 0, n_single_part = 0;
   bool by_blocks = false;  // cut_block_schedule made it: the lanes of a group read the same pages side by side
   bool tiles_in_l2 = false;  // most reads of a cache tile are answered by L2
+  int n_epochs = 1;          // > 1: cut_epoch_schedule made it
+  // E4M3 pages that are read many times over are turned into bf16 once per layer call (0: none): the pages, and the
+  // block tables with page numbers of the scratch pool in place of the pool's
+  int n_expand = 0;
+  int32_t *d_xpages = nullptr, *d_xtables = nullptr;
   // what the compressor kernel of this class reads (classes 1, 2)
   CompressTok* d_ctoks = nullptr;
   CompressStep* d_csteps = nullptr;
@@ -103,6 +108,14 @@ constexpr int MAX_EVENT_SETS = 256;
 // 25 142 / 148, 32 154 and 162 / 156 and 159, 48 185 and 188 / 183 and 179, 64 223 and 235 / 215 and 217
 // (V4: 1 row 119 / 125, 25 151 / 151, 32 160 and 165 / 159 and 162, 64 229 and 233 / 220).
 constexpr int SMALL_OUT = 32;
+// Bytes of distinct cache pages that a call attends to up to which they stay in L2 (126 MB) while every query
+// token walks them in its own order: about half of it.
+constexpr long long L2_ROWS_BYTES = 64ll << 20;
+constexpr int MAX_EPOCHS = 8;
+// An E4M3 page that a call reads this many times is worth turning into bf16 once for all of them, up to this much
+// scratch memory.
+constexpr int EXPAND_READS = 8;
+constexpr long long EXPAND_BYTES = 256ll << 20;
 constexpr int ROWS_TMP = 2048;  // rows per turn of a host copy into or out of an E4M3 pool
 
 // Page-locked rows with an address on the device, or (false) neither: without them the output is copied
@@ -145,6 +158,8 @@ struct FstMlaCtx {
 
   // paged-cache bookkeeping (host)
   std::vector<int32_t> free_pages, free_seqs;
+  std::vector<int32_t> page_ref;  // sequences that hold a page (fst_cuda_mla_seq_fork shares whole pages); 0: free
+  int n_shared = 0;               // pages held by more than one
   std::vector<std::vector<int32_t>> tables;
   std::vector<int32_t> lens;
   std::vector<char> live;
@@ -154,8 +169,13 @@ struct FstMlaCtx {
   bf16 *d_h = nullptr, *d_cmp = nullptr, *d_qc = nullptr, *d_kvnew = nullptr, *d_qfull = nullptr;
   bf16 *d_qeff = nullptr, *d_olat = nullptr, *d_low = nullptr, *d_out = nullptr;
   float *d_part_m = nullptr, *d_part_l = nullptr, *d_part_o = nullptr;
-  int max_parts = 0;
+  int max_parts = 0, max_parts0 = 0;  // partials there is room for; at the start
   bool fused_merge = true;       // the attention kernel finishes single-partial tokens itself
+  bool shared_prefix = true;     // plans take sequences that share pages together
+  std::vector<void*> retired;    // device memory that a captured graph may still name: kept until the context goes
+  std::vector<int32_t> page_mark;  // per page: its number among the distinct pages of the plan being built
+  bf16* d_expand = nullptr;      // scratch pool of expanded E4M3 pages
+  int expand_cap = 0;            // ... in pages
   bool block_schedule = true;    // calls with G >= 4 new tokens per sequence: thread blocks in groups of G lanes
   Sched sched[N_CLASSES];        // the current plan's schedule per layer class
   int info_class = 0;            // class of the layer that ran last (plan_info reports its schedule)
@@ -321,6 +341,21 @@ int cmp_width(const FstMlaCtx* c, int ratio) { return ratio == 4 ? 2 * c->d.kv_l
 int cmp_rows(int ratio) { return ratio == 4 ? 8 : ratio; }
 size_t cmp_slot_floats(const FstMlaCtx* c, int ratio) { return (size_t)2 * cmp_rows(ratio) * cmp_width(c, ratio); }
 
+int32_t take_page(FstMlaCtx* c) {
+  const int32_t pg = c->free_pages.back();
+  c->free_pages.pop_back();
+  c->page_ref[pg] = 1;
+  return pg;
+}
+void share_page(FstMlaCtx* c, int32_t pg) {
+  if (++c->page_ref[pg] == 2) ++c->n_shared;
+}
+void drop_page(FstMlaCtx* c, int32_t pg) {
+  const int left = --c->page_ref[pg];
+  if (left == 1) --c->n_shared;
+  if (left == 0) c->free_pages.push_back(pg);
+}
+
 bool seq_ok(const FstMlaCtx* c, int32_t s) { return s >= 0 && s < c->cfg.max_seqs && c->live[s]; }
 
 int reserve_pages(FstMlaCtx* c, int32_t seq, int32_t n_tokens) {
@@ -336,14 +371,8 @@ int reserve_pages(FstMlaCtx* c, int32_t seq, int32_t n_tokens) {
   if (more > c->free_pages.size())
     return fail(FST_MLA_ERR_PAGES, "page pool exhausted: sequence %d needs %zu more pages, %zu free", seq, more,
                 c->free_pages.size());
-  while (t.size() < need) {
-    t.push_back(c->free_pages.back());
-    c->free_pages.pop_back();
-  }
-  while (ct.size() < need_c) {
-    ct.push_back(c->free_pages.back());
-    c->free_pages.pop_back();
-  }
+  while (t.size() < need) t.push_back(take_page(c));
+  while (ct.size() < need_c) ct.push_back(take_page(c));
   c->lens[seq] = std::max(c->lens[seq], n_tokens);
   return FST_MLA_OK;
 }
@@ -356,6 +385,38 @@ long long pool_row(const FstMlaCtx* c, int32_t seq, int32_t pos) {
 long long row_offset(const FstMlaCtx* c, int32_t seq, int32_t pos) { return pool_row(c, seq, pos) * c->d.row; }
 PoolView view_of(const FstMlaCtx* c, int lid) {
   return pool_view(c->pools[lid], c->e4m3, c->d.row, c->d.rope, c->cfg.page_tokens);
+}
+
+// Copy on write: pages of rows [pos0, pos0 + n) that other sequences hold too become this sequence's own.  (A
+// shared page is full of rows that all its holders see: who is truncated into one has had it replaced.)
+int own_rows(FstMlaCtx* c, int32_t seq, int32_t pos0, int32_t n) {
+  if (c->n_shared == 0 || n <= 0) return FST_MLA_OK;
+  const int pt = c->cfg.page_tokens;
+  auto& t = c->tables[seq];
+  const int p0 = pos0 / pt, p1 = std::min<int>((pos0 + n - 1) / pt, (int)t.size() - 1);
+  size_t need = 0;
+  for (int p = p0; p <= p1; ++p) need += c->page_ref[t[p]] > 1;
+  if (need > c->free_pages.size())
+    return fail(FST_MLA_ERR_PAGES, "page pool exhausted: sequence %d writes into %zu shared pages, %zu free", seq, need,
+                c->free_pages.size());
+  for (int p = p0; p <= p1; ++p) {
+    const int32_t old = t[p];
+    if (c->page_ref[old] <= 1) continue;
+    const int32_t pg = take_page(c);
+    for (int l = 0; l < c->cfg.n_layers; ++l) {
+      cudaError_t e = launch_page_copy(view_of(c, l), old, pg, pt, c->stream);
+      if (e != cudaSuccess) {
+        drop_page(c, pg);
+        return fail(FST_MLA_ERR_CUDA, "page copy: %s", cudaGetErrorString(e));
+      }
+      c->launches += 1;
+    }
+    c->status_by_kernel = false;
+    t[p] = pg;
+    drop_page(c, old);
+    c->planned = false;
+  }
+  return FST_MLA_OK;
 }
 
 template <class T>
@@ -441,12 +502,30 @@ GemmArgs plain_gemm(const bf16* A, const bf16* B, bf16* C, int M, int N, int K) 
   return g;
 }
 
+// The plan blob.  First part: two RoPE tables, append addresses, per compressed class the compressor's inputs;
+// second part: per class (token partial ranges, block ranges, segments), then the block tables, and the pages
+// and tables of an expanded plan.  (Classes 1 and 2 have no epochs.)
+size_t plan_bytes(const FstMlaCtx* x) {
+  const size_t T = x->cfg.max_tokens;
+  return 2 * T * x->d.rope * sizeof(float) + T * sizeof(long long) +
+         2 * (T * sizeof(CompressTok) + (size_t)x->cfg.max_seqs * sizeof(CompressStep) + T * x->d.rope * sizeof(float)) +
+         N_CLASSES * ((T + 1) * sizeof(int32_t) + ((size_t)x->n_sm + 1) * sizeof(int32_t)) +
+         ((size_t)x->segs_cap + (N_CLASSES - 1) * (size_t)x->max_parts0) * sizeof(AttnSeg) +
+         (2 * (size_t)x->tables_cap + x->cfg.n_pages) * sizeof(int32_t) + 40 * 256;
+}
+
 AttnArgs attn_args(FstMlaCtx* c, int lid, const bf16* q_eff, bool may_fuse, bf16* o_lat) {
   AttnArgs a;
   a.q_eff = q_eff;
+  const Sched& S = sched_of(c, lid);
   a.pool = view_of(c, lid);
   a.tables = c->d_tables;
-  const Sched& S = sched_of(c, lid);
+  a.pool_rows = (long long)c->cfg.n_pages * c->cfg.page_tokens;
+  if (S.n_expand) {
+    a.pool = pool_view(c->d_expand, false, c->d.row, c->d.rope, c->cfg.page_tokens);
+    a.tables = S.d_xtables;
+    a.pool_rows = (long long)S.n_expand * c->cfg.page_tokens;
+  }
   a.segs = S.d_segs;
   a.cta_seg = S.d_cta_seg;
   a.part_m = c->d_part_m;
@@ -460,7 +539,6 @@ AttnArgs attn_args(FstMlaCtx* c, int lid, const bf16* q_eff, bool may_fuse, bf16
   a.d_v = c->d.d_v;
   a.row = c->d.row;
   a.page_tokens = c->cfg.page_tokens;
-  a.pool_rows = (long long)c->cfg.n_pages * c->cfg.page_tokens;
   a.q_rows = (long long)c->T * c->d.H;
   a.scale = c->cfg.softmax_scale;
   a.tiles_shared = S.tiles_in_l2;
@@ -490,6 +568,11 @@ int run_attention(FstMlaCtx* c, int lid, const bf16* q_eff, bool* direct = nullp
   if (direct) *direct = a.direct_single;
   if (c->cfg.attn_impl == FST_MLA_IMPL_TENSOR && !tc_ok)
     return fail(FST_MLA_ERR_ARG, "this shape has no tcgen05 attention path");
+  const Sched& S = sched_of(c, lid);
+  if (S.n_expand) {
+    CU(launch_expand_pages(view_of(c, lid), S.d_xpages, S.n_expand, c->d_expand, c->stream));
+    c->launches += 1;
+  }
   if (c->cfg.attn_impl != FST_MLA_IMPL_SIMT && tc_ok) {
     cudaError_t e = launch_attn_stream(a, c->stream);
     if (e != cudaSuccess) return fail(FST_MLA_ERR_CUDA, "tcgen05 attention launch: %s", cudaGetErrorString(e));
@@ -706,6 +789,7 @@ int fst_cuda_mla_create(const FstMlaConfig* cfg, FstMlaCtx** out) {
   x->layer_yarn.assign(c.n_layers, c.rope_yarn ? 1 : 0);
   x->pools.assign(c.n_layers, nullptr);
   for (int i = c.n_pages - 1; i >= 0; --i) x->free_pages.push_back(i);
+  x->page_ref.assign(c.n_pages, 0);
   for (int i = c.max_seqs - 1; i >= 0; --i) x->free_seqs.push_back(i);
   x->tables.resize(c.max_seqs);
   x->comp_tables.resize(c.max_seqs);
@@ -726,6 +810,7 @@ int fst_cuda_mla_create(const FstMlaConfig* cfg, FstMlaCtx** out) {
   // partials: one per thread block plus one per stream of tiles that starts inside a block's run; a
   // token has one stream, two in layers with a KV compressor (V4 form only)
   x->max_parts = x->n_sm + (int)T * (d.v4 ? 2 : 1);
+  x->max_parts0 = x->max_parts;
   if (!rc) rc = dev_alloc(&x->d_h, T * d.hidden);
   if (!rc) rc = dev_alloc(&x->d_cmp, T * d.cmp_n);
   if (!rc) rc = dev_alloc(&x->d_an, T * d.hidden);
@@ -740,15 +825,9 @@ int fst_cuda_mla_create(const FstMlaConfig* cfg, FstMlaCtx** out) {
   if (!rc) rc = dev_alloc(&x->d_part_m, (size_t)x->max_parts * d.H);
   if (!rc) rc = dev_alloc(&x->d_part_l, (size_t)x->max_parts * d.H);
   if (!rc) rc = dev_alloc(&x->d_part_o, (size_t)x->max_parts * d.H * d.d_v);
-  x->segs_cap = x->max_parts;
+  x->segs_cap = x->max_parts + (MAX_EPOCHS - 1) * (x->n_sm + (int)T);
   x->tables_cap = c.n_pages + c.max_seqs;
-  // first part: two RoPE tables, append addresses, per compressed class the compressor's inputs;
-  // second part: per class (token partial ranges, block ranges, segments), then the block tables
-  x->plan_cap = 2 * T * d.rope * sizeof(float) + T * sizeof(long long) +
-                2 * (T * sizeof(CompressTok) + (size_t)c.max_seqs * sizeof(CompressStep) + T * d.rope * sizeof(float)) +
-                N_CLASSES * ((T + 1) * sizeof(int32_t) + ((size_t)x->n_sm + 1) * sizeof(int32_t) +
-                             (size_t)x->segs_cap * sizeof(AttnSeg)) +
-                (size_t)x->tables_cap * sizeof(int32_t) + 32 * 256;
+  x->plan_cap = plan_bytes(x);
   if (!rc) rc = dev_alloc(&x->d_plan, x->plan_cap);
   if (!rc && cudaHostAlloc((void**)&x->h_plan, x->plan_cap, cudaHostAllocDefault) != cudaSuccess)
     rc = fail(FST_MLA_ERR_CUDA, "cudaHostAlloc(plan) failed");
@@ -798,6 +877,8 @@ void fst_cuda_mla_destroy(FstMlaCtx* c) {
   }
   cudaFree(c->d_cproj);
   for (auto p : c->pools) cudaFree(p);
+  for (void* q : c->retired) cudaFree(q);
+  cudaFree(c->d_expand);
   cudaFree(c->d_rows_tmp);
   cudaFree(c->d_runs);
   if (c->h_runs) cudaFreeHost(c->h_runs);
@@ -1043,30 +1124,53 @@ int fst_cuda_mla_seq_truncate(FstMlaCtx* c, int32_t seq, int32_t n_tokens) {
   if (n_tokens < 0 || n_tokens > c->lens[seq])
     return fail(FST_MLA_ERR_ARG, "truncate to %d outside [0, %d]", n_tokens, c->lens[seq]);
   CU(cudaSetDevice(c->cfg.device));
-  // zero the dropped rows in every layer, as the reference rollback does (6132-6147)
+  const int pt = c->cfg.page_tokens;
+  const size_t keep = ((size_t)n_tokens + pt - 1) / pt;
+  auto& t = c->tables[seq];
+  // a page that other sequences hold too and that would keep only some of its rows here is replaced by a copy
+  const bool split = n_tokens < c->lens[seq] && n_tokens % pt && c->page_ref[t[keep - 1]] > 1;
+  if (split) {
+    size_t back = c->free_pages.size();
+    for (size_t p = keep; p < t.size(); ++p) back += c->page_ref[t[p]] == 1;
+    if (back == 0) return fail(FST_MLA_ERR_PAGES, "page pool exhausted: row %d lies in a shared page", n_tokens);
+  }
+  // zero the dropped rows in every layer, as the reference rollback does (6132-6147); rows of shared pages are the others'
   const int n_drop = c->lens[seq] - n_tokens;
   if (n_drop > 0) {
-    std::vector<long long> offs(n_drop);
-    for (int i = 0; i < n_drop; ++i) offs[i] = c->e4m3 ? pool_row(c, seq, n_tokens + i) : row_offset(c, seq, n_tokens + i);
-    long long* d_offs = nullptr;
-    CU(cudaMalloc((void**)&d_offs, n_drop * sizeof(long long)));
-    cudaError_t e = cudaMemcpyAsync(d_offs, offs.data(), n_drop * sizeof(long long), cudaMemcpyHostToDevice, c->stream);
-    for (int l = 0; l < c->cfg.n_layers && e == cudaSuccess; ++l) {
-      if (c->e4m3)
-        launch_zero_rows_e4m3(view_of(c, l), d_offs, n_drop, c->stream);
-      else
-        launch_zero_rows(c->pools[l], d_offs, n_drop, c->d.row, c->stream);
+    std::vector<long long> offs;
+    offs.reserve(n_drop);
+    for (int i = 0; i < n_drop; ++i)
+      if (c->page_ref[t[(n_tokens + i) / pt]] == 1)
+        offs.push_back(c->e4m3 ? pool_row(c, seq, n_tokens + i) : row_offset(c, seq, n_tokens + i));
+    if (!offs.empty()) {
+      long long* d_offs = nullptr;
+      CU(cudaMalloc((void**)&d_offs, offs.size() * sizeof(long long)));
+      cudaError_t e = cudaMemcpyAsync(d_offs, offs.data(), offs.size() * sizeof(long long), cudaMemcpyHostToDevice, c->stream);
+      for (int l = 0; l < c->cfg.n_layers && e == cudaSuccess; ++l) {
+        if (c->e4m3)
+          launch_zero_rows_e4m3(view_of(c, l), d_offs, (int)offs.size(), c->stream);
+        else
+          launch_zero_rows(c->pools[l], d_offs, (int)offs.size(), c->d.row, c->stream);
+        c->launches += 1;
+      }
+      if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
+      cudaFree(d_offs);
+      if (e != cudaSuccess) return fail(FST_MLA_ERR_CUDA, "rollback failed: %s", cudaGetErrorString(e));
+    }
+  }
+  while (t.size() > keep) {
+    drop_page(c, t.back());
+    t.pop_back();
+  }
+  if (split) {
+    const int32_t old = t.back(), pg = take_page(c);
+    for (int l = 0; l < c->cfg.n_layers; ++l) {
+      CU(launch_page_copy(view_of(c, l), old, pg, n_tokens % pt, c->stream));
       c->launches += 1;
     }
-    if (e == cudaSuccess) e = cudaStreamSynchronize(c->stream);
-    cudaFree(d_offs);
-    if (e != cudaSuccess) return fail(FST_MLA_ERR_CUDA, "rollback failed: %s", cudaGetErrorString(e));
-  }
-  const size_t keep = ((size_t)n_tokens + c->cfg.page_tokens - 1) / c->cfg.page_tokens;
-  auto& t = c->tables[seq];
-  while (t.size() > keep) {
-    c->free_pages.push_back(t.back());
-    t.pop_back();
+    c->status_by_kernel = false;
+    t.back() = pg;
+    drop_page(c, old);
   }
   if (c->has_cmp) {
     // The compressed rows emitted by the dropped rows go with them.  The window state comes back
@@ -1075,7 +1179,7 @@ int fst_cuda_mla_seq_truncate(FstMlaCtx* c, int32_t seq, int32_t n_tokens) {
     const size_t keep_c = ((size_t)(n_tokens / c->cmp_min_ratio) + c->cfg.page_tokens - 1) / c->cfg.page_tokens;
     auto& ct = c->comp_tables[seq];
     while (ct.size() > keep_c) {
-      c->free_pages.push_back(ct.back());
+      drop_page(c, ct.back());
       ct.pop_back();
     }
     const bool restore = c->snap_len[seq] == n_tokens;
@@ -1094,6 +1198,49 @@ int fst_cuda_mla_seq_truncate(FstMlaCtx* c, int32_t seq, int32_t n_tokens) {
     if (n_tokens < c->snap_len[seq]) c->snap_len[seq] = -1;
   }
   c->lens[seq] = n_tokens;
+  c->planned = false;
+  return FST_MLA_OK;
+}
+
+int fst_cuda_mla_seq_fork(FstMlaCtx* c, int32_t src, int32_t n_tokens, int32_t* seq_out) {
+  if (!c || !seq_out) return fail(FST_MLA_ERR_ARG, "null argument");
+  if (!seq_ok(c, src)) return fail(FST_MLA_ERR_ARG, "sequence %d is not allocated", src);
+  if (n_tokens < 0 || n_tokens > c->lens[src]) return fail(FST_MLA_ERR_ARG, "fork at %d outside [0, %d]", n_tokens, c->lens[src]);
+  if (c->has_cmp) return fail(FST_MLA_ERR_STATE, "a KV compressor's window state belongs to one sequence: no forks");
+  if (c->free_seqs.empty()) return fail(FST_MLA_ERR_CAPACITY, "all %d sequence slots are in use", c->cfg.max_seqs);
+  const int pt = c->cfg.page_tokens, whole = n_tokens / pt, rest = n_tokens % pt;
+  if (rest && c->free_pages.empty())
+    return fail(FST_MLA_ERR_PAGES, "page pool exhausted: the fork's last page needs a copy");
+  CU(cudaSetDevice(c->cfg.device));
+  try {
+    std::vector<int32_t> table(c->tables[src].begin(), c->tables[src].begin() + whole);
+    table.reserve(whole + 1);
+    if (rest) {
+      // the last page goes on differently in the two: the fork gets a copy of its rows
+      const int32_t old = c->tables[src][whole], pg = take_page(c);
+      for (int l = 0; l < c->cfg.n_layers; ++l) {
+        cudaError_t e = launch_page_copy(view_of(c, l), old, pg, rest, c->stream);
+        if (e != cudaSuccess) {
+          drop_page(c, pg);
+          return fail(FST_MLA_ERR_CUDA, "page copy: %s", cudaGetErrorString(e));
+        }
+        c->launches += 1;
+      }
+      c->status_by_kernel = false;
+      table.push_back(pg);
+    }
+    const int s = c->free_seqs.back();
+    c->free_seqs.pop_back();
+    for (int p = 0; p < whole; ++p) share_page(c, table[p]);
+    c->live[s] = 1;
+    c->lens[s] = n_tokens;
+    c->tables[s].swap(table);
+    c->comp_tables[s].clear();
+    c->snap_len[s] = -1;
+    *seq_out = s;
+  } catch (const std::bad_alloc&) {
+    return fail(FST_MLA_ERR_CAPACITY, "out of host memory");
+  }
   c->planned = false;
   return FST_MLA_OK;
 }
@@ -1128,6 +1275,8 @@ int fst_cuda_mla_reset(FstMlaCtx* c) {
   c->free_pages.clear();
   c->free_seqs.clear();
   for (int i = c->cfg.n_pages - 1; i >= 0; --i) c->free_pages.push_back(i);
+  std::fill(c->page_ref.begin(), c->page_ref.end(), 0);
+  c->n_shared = 0;
   for (int i = c->cfg.max_seqs - 1; i >= 0; --i) c->free_seqs.push_back(i);
   for (auto& t : c->tables) t.clear();
   for (auto& t : c->comp_tables) t.clear();
@@ -1179,6 +1328,7 @@ static int cache_copy(FstMlaCtx* c, int lid, int32_t seq, int32_t pos0, int32_t 
   CU(cudaSetDevice(c->cfg.device));
   if (write) {
     int rc = reserve_pages(c, seq, pos0 + n);
+    if (!rc) rc = own_rows(c, seq, pos0, n);
     if (rc) return rc;
     c->planned = false;
   } else if (pos0 + n > c->lens[seq]) {
@@ -1419,6 +1569,7 @@ int plan_tokens_part(FstMlaCtx* c, const FstMlaSeqStep* steps, int32_t n_seqs, i
       return fail(FST_MLA_ERR_ARG, "step %d: rows [0, %d) are not all cached (length %d)", b, need, c->lens[s.seq]);
     if (s.append) {
       int rc = reserve_pages(c, s.seq, need);
+      if (!rc) rc = own_rows(c, s.seq, s.pos0, s.q_len);
       if (rc) return rc;
     }
   }
@@ -1458,7 +1609,26 @@ int plan_tokens_part(FstMlaCtx* c, const FstMlaSeqStep* steps, int32_t n_seqs, i
       kvlo[t] = s.window > 0 ? std::max(0, len - s.window) : 0;
     }
   }
-  if ((int)tables.size() > c->tables_cap) return fail(FST_MLA_ERR_CAPACITY, "block tables overflow");
+  if ((int)tables.size() > c->tables_cap) {
+    // sequences that share pages name them once each
+    CU(cudaStreamSynchronize(c->stream));
+    CU(cudaStreamSynchronize(c->copy_stream));
+    const int old_cap = c->tables_cap;
+    c->tables_cap = (int)std::min<size_t>(2 * tables.size(), 1u << 30);
+    const size_t bytes = plan_bytes(c);
+    unsigned char *d = nullptr, *h = nullptr;
+    if (cudaMalloc((void**)&d, bytes) != cudaSuccess || cudaHostAlloc((void**)&h, bytes, cudaHostAllocDefault) != cudaSuccess) {
+      cudaGetLastError();
+      cudaFree(d);
+      c->tables_cap = old_cap;
+      return fail(FST_MLA_ERR_CAPACITY, "no memory for block tables of %zu pages", tables.size());
+    }
+    c->retired.push_back(c->d_plan);
+    cudaFreeHost(c->h_plan);
+    c->d_plan = d;
+    c->h_plan = h;
+    c->plan_cap = bytes;
+  }
   c->pl_steps.assign(steps, steps + n_seqs);
   c->pl_causal = causal;
   c->T = (int)T;
@@ -1674,6 +1844,175 @@ bool cut_block_schedule(const FstMlaCtx* c, int T, std::vector<AttnSeg>* segs_ou
   return true;
 }
 
+// Sequences of the plan that share their first pages.  Fills group_of[step] (-1: alone) and, per group, the number
+// of pages that all its members begin with.
+struct PrefixGroups {
+  std::vector<int> group_of, pages, tokens;
+};
+void find_prefix_groups(const FstMlaCtx* c, PrefixGroups* out) {
+  const int n = (int)c->pl_steps.size();
+  out->group_of.assign(n, -1);
+  out->pages.clear();
+  out->tokens.clear();
+  std::vector<int> first;                         // the member each group is compared with
+  std::vector<std::pair<int32_t, int>> by_page;   // (first page, step), sorted: members side by side
+  for (int b = 0; b < n; ++b) {
+    const FstMlaSeqStep& st = c->pl_steps[b];
+    const auto& t = c->tables[st.seq];
+    if (st.q_len > 0 && st.window <= 0 && !t.empty() && c->page_ref[t[0]] > 1) by_page.emplace_back(t[0], b);
+  }
+  std::sort(by_page.begin(), by_page.end());
+  for (size_t i = 0; i < by_page.size();) {
+    size_t j = i;
+    while (j < by_page.size() && by_page[j].first == by_page[i].first) ++j;
+    if (j - i >= 2) {
+      const auto& t0 = c->tables[c->pl_steps[by_page[i].second].seq];
+      size_t common = t0.size();
+      int toks = 0;
+      for (size_t k = i; k < j; ++k) {
+        const FstMlaSeqStep& st = c->pl_steps[by_page[k].second];
+        const auto& t = c->tables[st.seq];
+        common = std::min(common, t.size());
+        for (size_t q = 0; q < common; ++q)
+          if (t[q] != t0[q]) common = q;
+        toks += st.q_len;
+      }
+      for (size_t k = i; k < j; ++k) out->group_of[by_page[k].second] = (int)out->pages.size();
+      out->pages.push_back((int)common);
+      out->tokens.push_back(toks);
+    }
+    i = j;
+  }
+}
+
+// The schedule for a batch over a shared prefix that L2 does not hold.  Cut token by token, the blocks would be
+// at as many places of the prefix at once as there are tokens, and every page would come from HBM once per
+// token.  Here the prefix is cut into EPOCHS of pages that do stay in L2; each epoch is cut over all blocks as the
+// token schedule cuts a batch, and a block walks its share of one epoch after the other, so that all
+// of them are in the same epoch at about the same time.  The price is partials: up to n_sm + T per epoch.  What a
+// token sees behind the prefix belongs to the last epoch (its rows go on in the same table).
+// Returns the number of epochs, or 0 (nothing written) when no group's prefix is worth it.
+int cut_epoch_schedule(const FstMlaCtx* c, int T, const PrefixGroups& pg, std::vector<AttnSeg>* segs_out,
+                       std::vector<int32_t>* cta_seg_out, std::vector<int32_t>* tok_part_out, long long* kv_rows_out) {
+  constexpr int unit = 64;
+  if (c->cfg.page_tokens != unit) return 0;
+  int longest = 0;
+  for (size_t g = 0; g < pg.pages.size(); ++g) longest = std::max(longest, pg.pages[g]);
+  const long long bytes = longest * (long long)c->page_bytes;
+  const int n_ep = (int)std::min<long long>(MAX_EPOCHS, (bytes + L2_ROWS_BYTES * 3 / 4 - 1) / (L2_ROWS_BYTES * 3 / 4));
+  if (n_ep < 2) return 0;
+  const int per = (longest + n_ep - 1) / n_ep;  // pages of an epoch
+  std::vector<std::vector<AttnSeg>> eseg(n_ep);
+  std::vector<std::vector<int32_t>> ecta(n_ep);
+  std::vector<TileStream> streams;
+  std::vector<int32_t> unused;
+  int n_ctas = 0;
+  *kv_rows_out = 0;
+  for (int e = 0; e < n_ep; ++e) {
+    streams.clear();
+    for (int t = 0; t < T; ++t) {
+      const int g = pg.group_of[c->pl_tok_step[t]];
+      // a token's rows of this epoch: its group's pages [e * per, (e + 1) * per), and all that is left in its last
+      const int last = g < 0 ? 0 : std::max(0, (pg.pages[g] - 1) / per);
+      if (e > last) continue;
+      const int lo = std::max(c->pl_kvlo[t], e * per * unit);
+      const int hi = e == last ? c->pl_kvlen[t] : std::min(c->pl_kvlen[t], (e + 1) * per * unit);
+      if (hi > lo) streams.push_back(TileStream{t, c->pl_tok_table[t], lo, hi});
+    }
+    long long rows = 0;
+    cut_schedule(c, streams, T, &eseg[e], &ecta[e], &unused, &rows);
+    *kv_rows_out += rows;
+    n_ctas = std::max(n_ctas, (int)ecta[e].size() - 1);
+  }
+  std::vector<int32_t> parts_of(T, 0);
+  for (int e = 0; e < n_ep; ++e)
+    for (AttnSeg& sg : eseg[e]) sg.part = parts_of[sg.tok]++;
+  tok_part_out->assign(T + 1, 0);
+  for (int t = 0; t < T; ++t) (*tok_part_out)[t + 1] = (*tok_part_out)[t] + parts_of[t];
+  segs_out->clear();
+  cta_seg_out->assign(n_ctas + 1, 0);
+  for (int k = 0; k < n_ctas; ++k) {
+    (*cta_seg_out)[k] = (int)segs_out->size();
+    for (int e = 0; e < n_ep; ++e)
+      if (k + 1 < (int)ecta[e].size())
+        for (int i = ecta[e][k]; i < ecta[e][k + 1]; ++i) {
+          AttnSeg sg = eseg[e][i];
+          sg.part += (*tok_part_out)[sg.tok];
+          segs_out->push_back(sg);
+        }
+  }
+  (*cta_seg_out)[n_ctas] = (int)segs_out->size();
+  return n_ep;
+}
+
+// Room for n partials.  What was there stays allocated: a captured graph may still write to it.
+bool more_parts(FstMlaCtx* c, int n) {
+  if (n <= c->max_parts) return true;
+  float *m = nullptr, *l = nullptr, *o = nullptr;
+  const size_t H = c->d.H;
+  if (cudaMalloc((void**)&m, n * H * sizeof(float)) != cudaSuccess || cudaMalloc((void**)&l, n * H * sizeof(float)) != cudaSuccess ||
+      cudaMalloc((void**)&o, n * H * c->d.d_v * sizeof(float)) != cudaSuccess) {
+    cudaGetLastError();
+    cudaFree(m);
+    cudaFree(l);
+    cudaFree(o);
+    return false;
+  }
+  c->retired.push_back(c->d_part_m);
+  c->retired.push_back(c->d_part_l);
+  c->retired.push_back(c->d_part_o);
+  c->d_part_m = m;
+  c->d_part_l = l;
+  c->d_part_o = o;
+  c->max_parts = n;
+  return true;
+}
+
+// The distinct pages that the tokens of the plan see, and the plan's block tables with their numbers instead of
+// the pool's.  False (and the E4M3 pages are read as they are) where the kernel for 64 heads does not run or the
+// scratch pool would be too large or cannot be had.
+bool expand_pages(FstMlaCtx* c, std::vector<int32_t>* pages, std::vector<int32_t>* tables) {
+  const Dims& d = c->d;
+  const int pt = c->cfg.page_tokens;
+  if (c->cfg.attn_impl == FST_MLA_IMPL_SIMT || pt != 64 || d.H != 64 || d.d_v != 512 || d.rope != 64) return false;
+  const size_t page_bf16 = (size_t)pt * d.row * sizeof(bf16);
+  const int most = (int)(EXPAND_BYTES / page_bf16);
+  pages->clear();
+  tables->assign(c->pl_tables.size(), 0);
+  c->page_mark.assign(c->cfg.n_pages, -1);
+  for (int t = 0; t < c->T; ++t) {
+    if (c->pl_kvlen[t] <= c->pl_kvlo[t]) continue;
+    const int off = c->pl_tok_table[t];
+    // (the tokens of a step see nested ranges of one table: what the token before has numbered is passed over)
+    int p0 = c->pl_kvlo[t] / pt;
+    const int p1 = (c->pl_kvlen[t] - 1) / pt;
+    if (t > 0 && c->pl_tok_table[t - 1] == off && c->pl_kvlo[t - 1] <= c->pl_kvlo[t]) p0 = std::max(p0, (c->pl_kvlen[t - 1] + pt - 1) / pt - 1);
+    for (int p = std::max(p0, 0); p <= p1; ++p) {
+      const int32_t pg = c->pl_tables[off + p];
+      if (c->page_mark[pg] < 0) {
+        if ((int)pages->size() == most) return false;
+        c->page_mark[pg] = (int)pages->size();
+        pages->push_back(pg);
+      }
+      (*tables)[off + p] = c->page_mark[pg];
+    }
+  }
+  const int n = (int)pages->size();
+  if (n == 0) return false;
+  if (n > c->expand_cap) {
+    const int cap = std::min(most, std::max(2 * n, 256));
+    bf16* x = nullptr;
+    if (cudaMalloc((void**)&x, cap * page_bf16) != cudaSuccess) {
+      cudaGetLastError();
+      return false;
+    }
+    if (c->d_expand) c->retired.push_back(c->d_expand);
+    c->d_expand = x;
+    c->expand_cap = cap;
+  }
+  return true;
+}
+
 // The second part: schedules (one per layer class in use) and block tables.  on_copy_stream:
 // upload it beside the kernels that already run on the context's stream (which then waits for
 // it); else one copy of the whole blob (or of the second part, if the first went ahead) on the
@@ -1695,7 +2034,7 @@ int plan_schedule_part(FstMlaCtx* c, bool on_copy_stream) {
   for (const LayerW& l : c->layers) in_use[class_of_ratio(l.cmp_ratio)] = true;
   std::vector<TileStream> streams;
   std::vector<AttnSeg> segs;
-  std::vector<int32_t> cta_seg, tok_part;
+  std::vector<int32_t> cta_seg, tok_part, xpages, xtables;
   for (int k = 0; k < N_CLASSES; ++k) {
     Sched& S = c->sched[k];
     S.built = false;
@@ -1720,8 +2059,30 @@ int plan_schedule_part(FstMlaCtx* c, bool on_copy_stream) {
       }
     }
     long long kv_rows = 0;
+    // distinct rows that the call attends to
+    long long rows_once = 0;
+    const bool sharing = k == 0 && c->shared_prefix && c->n_shared > 0;
+    PrefixGroups pg;
+    if (sharing) find_prefix_groups(c, &pg);
+    for (size_t b = 0; b < c->pl_steps.size(); ++b) {
+      const FstMlaSeqStep& step = c->pl_steps[b];
+      if (step.q_len > 0) rows_once += step.append ? step.pos0 + step.q_len : step.pos0;
+    }
+    if (!pg.pages.empty())
+      for (size_t g = 0; g < pg.pages.size(); ++g) {
+        long long members = 0;
+        for (int x : pg.group_of) members += x == (int)g;
+        rows_once = std::max(1ll, rows_once - (members - 1) * pg.pages[g] * (long long)c->cfg.page_tokens);
+      }
     S.by_blocks = k == 0 && c->block_schedule && cut_block_schedule(c, T, &segs, &cta_seg, &tok_part, &kv_rows);
-    if (!S.by_blocks) cut_schedule(c, streams, T, &segs, &cta_seg, &tok_part, &kv_rows);
+    S.n_epochs = 1;
+    if (!S.by_blocks) {
+      if (!pg.pages.empty() && rows_once / c->cfg.page_tokens * (long long)c->page_bytes > L2_ROWS_BYTES) {
+        const int n = cut_epoch_schedule(c, T, pg, &segs, &cta_seg, &tok_part, &kv_rows);
+        if (n > 0 && (int)segs.size() <= c->segs_cap && more_parts(c, (int)segs.size())) S.n_epochs = n;
+      }
+      if (S.n_epochs == 1) cut_schedule(c, streams, T, &segs, &cta_seg, &tok_part, &kv_rows);
+    }
     if ((int)segs.size() > c->segs_cap || (int)segs.size() > c->max_parts)
       return fail(FST_MLA_ERR_CAPACITY, "split schedule overflow");
     S.d_tok_part = reinterpret_cast<int32_t*>(put(tok_part.data(), (size_t)(T + 1) * sizeof(int32_t)));
@@ -1743,13 +2104,16 @@ int plan_schedule_part(FstMlaCtx* c, bool on_copy_stream) {
     // 232 / 225), 1300 rows 477 / 467 (V4 605 / 602), 12 blocks of 9-14 behind 1200 131 / 128; with fewer
     // than ten tiles per block (verify blocks of 5 to 16 rows over some hundred) within what two
     // processes of one build differ by.
-    long long rows_once = 0;
-    for (const FstMlaSeqStep& step : c->pl_steps)
-      if (step.q_len > 0) rows_once += step.append ? step.pos0 + step.q_len : step.pos0;
-    S.tiles_in_l2 = S.by_blocks || (kv_rows >= 4 * rows_once && rows_once / c->cfg.page_tokens * (long long)c->page_bytes <= (64ll << 20));
+    S.tiles_in_l2 = S.by_blocks || S.n_epochs > 1 || (kv_rows >= 4 * rows_once && rows_once / c->cfg.page_tokens * (long long)c->page_bytes <= L2_ROWS_BYTES);
     S.n_segs = S.n_parts = (int)segs.size();
     S.n_ctas = (int)cta_seg.size() - 1;
     S.kv_rows = kv_rows;
+    S.n_expand = 0;
+    if (k == 0 && c->e4m3 && kv_rows >= EXPAND_READS * rows_once && expand_pages(c, &xpages, &xtables)) {
+      S.n_expand = (int)xpages.size();
+      S.d_xpages = reinterpret_cast<int32_t*>(put(xpages.data(), xpages.size() * sizeof(int32_t)));
+      S.d_xtables = reinterpret_cast<int32_t*>(put(xtables.data(), xtables.size() * sizeof(int32_t)));
+    }
     S.built = true;
   }
   c->d_tables = reinterpret_cast<int32_t*>(put(tables.data(), tables.size() * sizeof(int32_t)));
@@ -1794,6 +2158,13 @@ int fst_cuda_mla_set_block_schedule(FstMlaCtx* c, int32_t on) {
   if (!c) return fail(FST_MLA_ERR_ARG, "null context");
   if (c->block_schedule != (on != 0)) c->planned = false;  // the next call builds its plan anew
   c->block_schedule = on != 0;
+  return FST_MLA_OK;
+}
+
+int fst_cuda_mla_set_shared_prefix(FstMlaCtx* c, int32_t on) {
+  if (!c) return fail(FST_MLA_ERR_ARG, "null context");
+  if (c->shared_prefix != (on != 0)) c->planned = false;
+  c->shared_prefix = on != 0;
   return FST_MLA_OK;
 }
 

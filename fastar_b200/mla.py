@@ -117,6 +117,8 @@ def load_library() -> C.CDLL:
     L.fst_cuda_mla_cache_write.argtypes = [vp, C.c_int, i32, i32, i32, u16p]
     L.fst_cuda_mla_cache_read.argtypes = [vp, C.c_int, i32, i32, i32, u16p]
     L.fst_cuda_mla_pool_read.argtypes = [vp, C.c_int, u16p, C.c_size_t]
+    L.fst_cuda_mla_seq_fork.argtypes = [vp, i32, i32, i32p]
+    L.fst_cuda_mla_set_shared_prefix.argtypes = [vp, i32]
     L.fst_cuda_mla_set_cache_format.argtypes = [vp, i32]
     L.fst_cuda_mla_cache_page_bytes.argtypes = [vp, C.POINTER(i64)]
     L.fst_cuda_mla_cache_append_device.argtypes = [vp, C.c_int, vp]
@@ -318,6 +320,12 @@ class MlaContext:
     def seq_free(self, seq: int) -> None:
         self._check(self.lib.fst_cuda_mla_seq_free(self._h, seq))
 
+    def seq_fork(self, src: int, n_tokens: int) -> int:
+        """A new sequence that begins with the first n_tokens rows of src, its whole pages shared."""
+        s = C.c_int32()
+        self._check(self.lib.fst_cuda_mla_seq_fork(self._h, src, n_tokens, C.byref(s)))
+        return s.value
+
     def seq_reserve(self, seq: int, n: int) -> None:
         self._check(self.lib.fst_cuda_mla_seq_reserve(self._h, seq, n))
 
@@ -406,6 +414,10 @@ class MlaContext:
     def set_block_schedule(self, on: bool) -> None:
         """Calls with G >= 4 new tokens per sequence: thread blocks in groups of G lanes that share pages."""
         self._check(self.lib.fst_cuda_mla_set_block_schedule(self._h, 1 if on else 0))
+
+    def set_shared_prefix(self, on: bool) -> None:
+        """Plans take sequences that share pages together (default)."""
+        self._check(self.lib.fst_cuda_mla_set_shared_prefix(self._h, 1 if on else 0))
 
     def set_fused_merge(self, on: bool) -> None:
         """Let the attention kernel finish tokens that have a single partial itself (default)."""

@@ -211,6 +211,16 @@ int fst_cuda_mla_seq_snapshot(FstMlaCtx* ctx, int32_t seq);
  * pool; pages come from a LIFO free list that initially hands out 0, 1, 2, ... */
 int fst_cuda_mla_seq_alloc(FstMlaCtx* ctx, int32_t* seq_out);
 int fst_cuda_mla_seq_free(FstMlaCtx* ctx, int32_t seq);
+/* A new sequence that begins with the first n_tokens rows of `src`, in every layer: a prompt, a document or a chat that
+ * several sequences go on from.  Whole pages are shared, not copied, and the rows of a page that n_tokens ends
+ * inside are copied (one page per layer): a fork takes one page at most, whatever its length.  From then on the
+ * two are sequences of their own: each appends, is truncated and freed by itself, a page returns to the
+ * pool with its last holder, a call that writes into a shared page (cache_write, a plan step with append = 1 over
+ * rows that are there) gets copies of the pages it touches first, and a truncation that ends inside a shared page
+ * takes a copy of what stays.  FST_MLA_ERR_PAGES when no page is left for such a copy (nothing has changed then).
+ * A plan that holds sequences with the same first pages reads these once for all, see
+ * fst_cuda_mla_set_shared_prefix.  Not in contexts with a KV compressor (FST_MLA_ERR_STATE). */
+int fst_cuda_mla_seq_fork(FstMlaCtx* ctx, int32_t src, int32_t n_tokens, int32_t* seq_out);
 /* Grow the table to hold n_tokens (no-op if it already does). */
 int fst_cuda_mla_seq_reserve(FstMlaCtx* ctx, int32_t seq, int32_t n_tokens);
 /* Speculative-decoding rollback (src/fst_engine.cpp:6132-6147): drop rows >= n_tokens,
@@ -280,6 +290,12 @@ int fst_cuda_mla_set_fused_merge(FstMlaCtx* ctx, int32_t on);
  * decode for every call.  Results do not depend on it beyond the order of a token's parts.
  * Default: on. */
 int fst_cuda_mla_set_block_schedule(FstMlaCtx* ctx, int32_t on);
+/* Calls in which sequences share pages (fst_cuda_mla_seq_fork): the plan counts what the batch reads by distinct
+ * pages.  A prefix that stays in L2 is walked token by token with the tiles kept there; a longer one in epochs,
+ * stretches of pages that do stay there and that all thread blocks walk at about the same time, so that each
+ * page comes from HBM once.  on = 0: scheduled as if nothing were shared.  Results do not depend on it beyond the order
+ * in which a token's parts are added.  Default: on. */
+int fst_cuda_mla_set_shared_prefix(FstMlaCtx* ctx, int32_t on);
 /* Sliding window that fst_cuda_mla_forward applies to every sequence of its calls (0: none). */
 int fst_cuda_mla_set_window(FstMlaCtx* ctx, int32_t window);
 /* Plans built and plan requests answered by the valid plan, since the context was created. */

@@ -111,10 +111,19 @@ constexpr int SMALL_OUT = 32;
 // Bytes of distinct cache pages that a call attends to up to which they stay in L2 (126 MB) while every query
 // token walks them in its own order: about half of it.
 constexpr long long L2_ROWS_BYTES = 64ll << 20;
+// A shared prefix that does not stay there is walked in epochs of 48 MiB from this many reads of a page on.  With /
+// without epochs, us, bf16: 4 users over 130 000 rows 115 / 101, 12 users 264 / 308, 24 users 487 / 561, 100 users over
+// 62 000 rows 924 / 1128; E4M3, 6 users over 130 000 rows 183 / 178.  Epochs of 24 MiB: 24 users 520; of 80 MiB:
+// 496, and 64 users over 62 000 rows (71 MB, then one epoch) 718 against 601.
+constexpr int EPOCH_READS = 8;
+constexpr long long EPOCH_BYTES = 48ll << 20;
 constexpr int MAX_EPOCHS = 8;
-// An E4M3 page that a call reads this many times is worth turning into bf16 once for all of them, up to this much
-// scratch memory.
-constexpr int EXPAND_READS = 8;
+// An E4M3 page that a call reads this many times is worth turning into bf16 once for all of them (the kernel that
+// dequantises takes 3500 cycles a tile, the bf16 one 2600; the expansion itself 23 us for 64 000 rows), up to this
+// much scratch memory.  Expanded / not, us: 8 x 16 new tokens over 8000 rows 198 / 226, 16 forks of 8000 rows 45.7 / 47.4,
+// 64 forks 98.6 / 119.3, a prompt of 2000 rows 365 / 500; 12 forks 41.5 / 41.5; 8 x 8 x 8000 121.2 / 119.7, 8 forks
+// 33.2 / 31.1, 8 x 4 x 8000 84.4 / 67.7.
+constexpr int EXPAND_READS = 10;
 constexpr long long EXPAND_BYTES = 256ll << 20;
 constexpr int ROWS_TMP = 2048;  // rows per turn of a host copy into or out of an E4M3 pool
 
@@ -1892,14 +1901,14 @@ void find_prefix_groups(const FstMlaCtx* c, PrefixGroups* out) {
 // of them are in the same epoch at about the same time.  The price is partials: up to n_sm + T per epoch.  What a
 // token sees behind the prefix belongs to the last epoch (its rows go on in the same table).
 // Returns the number of epochs, or 0 (nothing written) when no group's prefix is worth it.
-int cut_epoch_schedule(const FstMlaCtx* c, int T, const PrefixGroups& pg, std::vector<AttnSeg>* segs_out,
+int cut_epoch_schedule(const FstMlaCtx* c, int T, const PrefixGroups& pg, long long page_bytes, std::vector<AttnSeg>* segs_out,
                        std::vector<int32_t>* cta_seg_out, std::vector<int32_t>* tok_part_out, long long* kv_rows_out) {
   constexpr int unit = 64;
   if (c->cfg.page_tokens != unit) return 0;
   int longest = 0;
   for (size_t g = 0; g < pg.pages.size(); ++g) longest = std::max(longest, pg.pages[g]);
-  const long long bytes = longest * (long long)c->page_bytes;
-  const int n_ep = (int)std::min<long long>(MAX_EPOCHS, (bytes + L2_ROWS_BYTES * 3 / 4 - 1) / (L2_ROWS_BYTES * 3 / 4));
+  const long long bytes = longest * page_bytes;
+  const int n_ep = (int)std::min<long long>(MAX_EPOCHS, (bytes + EPOCH_BYTES - 1) / EPOCH_BYTES);
   if (n_ep < 2) return 0;
   const int per = (longest + n_ep - 1) / n_ep;  // pages of an epoch
   std::vector<std::vector<AttnSeg>> eseg(n_ep);
@@ -2074,11 +2083,20 @@ int plan_schedule_part(FstMlaCtx* c, bool on_copy_stream) {
         for (int x : pg.group_of) members += x == (int)g;
         rows_once = std::max(1ll, rows_once - (members - 1) * pg.pages[g] * (long long)c->cfg.page_tokens);
       }
+    // E4M3 pages that are read often are expanded: the attention then reads bf16 pages of a scratch pool
+    long long pairs = 0, page_read = (long long)c->page_bytes;
+    for (int t = 0; t < T; ++t) pairs += std::max(0, kvlen[t] - kvlo[t]);
+    S.n_expand = 0;
+    if (k == 0 && c->e4m3 && pairs >= EXPAND_READS * rows_once && expand_pages(c, &xpages, &xtables)) {
+      S.n_expand = (int)xpages.size();
+      page_read = (long long)c->cfg.page_tokens * c->d.row * (long long)sizeof(bf16);
+    }
+    const bool stays_in_l2 = rows_once / c->cfg.page_tokens * page_read <= L2_ROWS_BYTES;
     S.by_blocks = k == 0 && c->block_schedule && cut_block_schedule(c, T, &segs, &cta_seg, &tok_part, &kv_rows);
     S.n_epochs = 1;
     if (!S.by_blocks) {
-      if (!pg.pages.empty() && rows_once / c->cfg.page_tokens * (long long)c->page_bytes > L2_ROWS_BYTES) {
-        const int n = cut_epoch_schedule(c, T, pg, &segs, &cta_seg, &tok_part, &kv_rows);
+      if (!pg.pages.empty() && !stays_in_l2 && pairs >= EPOCH_READS * rows_once) {
+        const int n = cut_epoch_schedule(c, T, pg, page_read, &segs, &cta_seg, &tok_part, &kv_rows);
         if (n > 0 && (int)segs.size() <= c->segs_cap && more_parts(c, (int)segs.size())) S.n_epochs = n;
       }
       if (S.n_epochs == 1) cut_schedule(c, streams, T, &segs, &cta_seg, &tok_part, &kv_rows);
@@ -2104,13 +2122,11 @@ int plan_schedule_part(FstMlaCtx* c, bool on_copy_stream) {
     // 232 / 225), 1300 rows 477 / 467 (V4 605 / 602), 12 blocks of 9-14 behind 1200 131 / 128; with fewer
     // than ten tiles per block (verify blocks of 5 to 16 rows over some hundred) within what two
     // processes of one build differ by.
-    S.tiles_in_l2 = S.by_blocks || S.n_epochs > 1 || (kv_rows >= 4 * rows_once && rows_once / c->cfg.page_tokens * (long long)c->page_bytes <= L2_ROWS_BYTES);
+    S.tiles_in_l2 = S.by_blocks || S.n_epochs > 1 || (kv_rows >= 4 * rows_once && stays_in_l2);
     S.n_segs = S.n_parts = (int)segs.size();
     S.n_ctas = (int)cta_seg.size() - 1;
     S.kv_rows = kv_rows;
-    S.n_expand = 0;
-    if (k == 0 && c->e4m3 && kv_rows >= EXPAND_READS * rows_once && expand_pages(c, &xpages, &xtables)) {
-      S.n_expand = (int)xpages.size();
+    if (S.n_expand) {
       S.d_xpages = reinterpret_cast<int32_t*>(put(xpages.data(), xpages.size() * sizeof(int32_t)));
       S.d_xtables = reinterpret_cast<int32_t*>(put(xtables.data(), xtables.size() * sizeof(int32_t)));
     }

@@ -293,6 +293,14 @@ int FSTEngine::new_sequence() {
   return s;
 }
 
+int FSTEngine::fork_sequence(int seq, int n) {
+  int32_t s = -1;
+  check(fst_cuda_mla_seq_fork(ctx_, seq, n, &s), "seq_fork");
+  return s;
+}
+
+void FSTEngine::set_cache_format(int format) { check(fst_cuda_mla_set_cache_format(ctx_, format), "set_cache_format"); }
+
 void FSTEngine::free_sequence(int seq) { check(fst_cuda_mla_seq_free(ctx_, seq), "seq_free"); }
 
 std::vector<RandmatResult> FSTEngine::randmat_test() {

@@ -109,6 +109,12 @@ int fst_engine_new_sequence(FSTEngine* e) {
   guard([&] { s = e->new_sequence(); });
   return s;
 }
+int fst_engine_fork_sequence(FSTEngine* e, int seq, int n) {
+  int s = -1;
+  guard([&] { s = e->fork_sequence(seq, n); });
+  return s;
+}
+int fst_engine_set_cache_format(FSTEngine* e, int format) { return guard([&] { e->set_cache_format(format); }); }
 int fst_engine_current_sequence(FSTEngine* e) { return e->current_sequence(); }
 // Fills cos / ratio / maxerr for up to cap probes; returns the number of probes or -1.
 int fst_engine_randmat_test(FSTEngine* e, double* cosine, double* ratio, double* max_err, int cap) {

@@ -385,3 +385,155 @@ def test_engine_with_forks_and_a_quantised_cache(preset):
         assert np.array_equal(ctx.forward(0, prompt, [a], [0], [75], causal=True), got)
         f = [a, ctx.seq_fork(a, 75), ctx.seq_fork(a, 64)]
         assert np.array_equal(ctx.forward(0, h, f, [75, 75, 64], [1, 1, 1]), step)
+
+
+def check_on_device(torch, ctx, steps, q, got, causal, sinks=None):
+    """check_attention in 64 bits on the device, for long contexts; the rows are read back from the cache."""
+    row = ctx.dims["row"]
+    v4 = ctx.cfg.preset == mla.PRESET_FASTAR_V4
+    qd = torch.from_numpy(q.view(np.int16)).cuda().view(torch.bfloat16).double().reshape(-1, 64, row)
+    gd = torch.from_numpy(f32(got).astype(np.float64)).cuda()
+    scale = mla.default_scale(ctx.cfg)
+    t = 0
+    for s, pos0, n, *more in steps:
+        own = not more or len(more) < 2 or more[1]
+        total = pos0 + (n if own else 0)
+        buf = torch.zeros(max(total, 1), row, dtype=torch.bfloat16, device="cuda")
+        ctx.cache_read_device(0, [(s, 0, total)], buf.data_ptr())
+        ctx.sync()
+        keys = buf.double()
+        for i in range(n):
+            k = keys[:(pos0 + i + 1 if causal else total)]
+            logits = qd[t] @ k.T * scale
+            if sinks is not None:
+                logits = torch.cat([logits, torch.from_numpy(sinks).cuda().double()[:, None]], 1)
+            p = torch.softmax(logits, 1)[:, :k.shape[0]]
+            o, a = p @ k[:, :512], p @ k[:, :512].abs()
+            tol = 2.0 ** -8 * a + 2.0 ** -8 * o.abs()
+            if v4:
+                tol = 2.0 ** -8 * a + 2.0 ** -7 * o.abs()
+                ang = (pos0 + i) * 10000.0 ** (-torch.arange(0, 64, 2, device="cuda", dtype=torch.float64) / 64)
+                x0, x1 = o[:, 448::2].clone(), o[:, 449::2].clone()
+                o[:, 448::2], o[:, 449::2] = x0 * ang.cos() + x1 * ang.sin(), x1 * ang.cos() - x0 * ang.sin()
+                pair = tol[:, 448:].reshape(64, 32, 2).sum(2).repeat_interleave(2, 1)
+                tol[:, 448:] = pair * (1 + 2.0 ** -12)
+                tol += 2.0 ** -11 * o.abs().max()
+            err = (gd[t] - o).abs()
+            assert bool((err <= tol).all()), (t, float((err / tol).max()))
+            t += 1
+
+
+def fill(torch, ctx, seq, n, gen, row, pos=0):
+    x = torch.randn(n, row, generator=gen, device="cuda").to(torch.bfloat16)
+    for i in range(0, n, 512):
+        ctx.plan([(seq, pos + i, min(512, n - i))])
+        ctx.cache_append_device(0, x[i:i + 512].data_ptr())
+    ctx.sync()
+
+
+LONG = [
+    # (prefix, users, rows of their own up to, new tokens, other sequences)
+    (6400, 30, 1, 1, 0),        # the shared pages are all but a row of it
+    (6400, 31, 200, 1, 2),      # an odd number of users, others beside them
+    (6401, 24, 70, 1, 0),       # a prefix that ends inside a page
+    (3000, 20, 90, 3, 1),       # blocks of new tokens on a shared prefix
+    (20000, 8, 300, 1, 0),
+]
+
+
+@pytest.mark.parametrize("e4m3", FORMATS)
+@pytest.mark.parametrize("preset", [mla.PRESET_BASELINE, mla.PRESET_FASTAR_V4])
+@pytest.mark.parametrize("prefix,users,own,q_len,others", LONG)
+def test_long_shared_prefix(torch, prefix, users, own, q_len, others, preset, e4m3):
+    rng = np.random.default_rng(8)
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(9)
+    v4 = preset == mla.PRESET_FASTAR_V4
+    with make(preset, e4m3=e4m3, n_pages=prefix // 64 + (users + others + 2) * 8, max_seqs=users + others + 1, max_tokens=512) as ctx:
+        row = ctx.dims["row"]
+        sinks = rng.standard_normal(64).astype(np.float32) if v4 else None
+        w = {n: np.zeros(sh, np.uint16) for n, sh in mla.weight_shapes(ctx.cfg).items()}
+        w["attn_sinks"] = sinks
+        ctx.set_layer_weights(0, w)
+        base = ctx.seq_alloc()
+        fill(torch, ctx, base, prefix, gen, row)
+        seqs = [ctx.seq_fork(base, prefix) for _ in range(users)]
+        steps = []
+        for i, s in enumerate(seqs):
+            n = 1 + (i * 37) % own
+            fill(torch, ctx, s, n - 1 + q_len, gen, row, prefix)
+            steps.append((s, prefix + n - 1, q_len))
+        for i in range(others):
+            s = ctx.seq_alloc()
+            fill(torch, ctx, s, 100 + 37 * i + 1, gen, row)
+            steps.insert(3 * i, (s, 100 + 37 * i, 1))
+        T = sum(s[2] for s in steps)
+        q = bits(rng.standard_normal((T * 64, row)).astype(np.float32) * (3.0 if v4 else 1.0))
+        got = run_batch(torch, ctx, steps, q, T, True)
+        check_on_device(torch, ctx, steps, q, got, True, sinks)
+        for _ in range(3):
+            assert np.array_equal(run_batch(torch, ctx, steps, q, T, True), got)
+
+
+@pytest.mark.parametrize("prefix,users", [(64, 2400), (130, 1301), (200, 900)])
+def test_many_users_of_a_page_or_two(torch, prefix, users):
+    """Segments of one, two and three tiles, many to a block; more users than thread blocks."""
+    rng = np.random.default_rng(13)
+    with make(e4m3=False, n_pages=users + 10, max_seqs=users + 1, max_tokens=users) as ctx:
+        base = ctx.seq_alloc()
+        ctx.cache_write(0, base, 0, rows_of(rng, prefix))
+        seqs = [ctx.seq_fork(base, prefix) for _ in range(users)]
+        steps = [(s, prefix, 1, -1, 0) for s in seqs]
+        q = bits(rng.standard_normal((users * 64, 576)).astype(np.float32))
+        launches = ctx.launch_count()
+        got = run_batch(torch, ctx, steps, q, users, False)
+        k = torch.from_numpy(f32(ctx.cache_read(0, base, 0, prefix)).astype(np.float64)).cuda()
+        qd = torch.from_numpy(q.view(np.int16)).cuda().view(torch.bfloat16).double()
+        p = torch.softmax(qd @ k.T * 192.0 ** -0.5, 1)
+        o, a = p @ k[:, :512], p @ k[:, :512].abs()
+        err = (torch.from_numpy(f32(got).astype(np.float64)).cuda().reshape(-1, 512) - o).abs()
+        assert bool((err <= 2.0 ** -8 * a + 2.0 ** -8 * o.abs()).all())
+        assert np.array_equal(run_batch(torch, ctx, steps, q, users, False), got)
+        assert ctx.launch_count() > launches
+
+
+@pytest.mark.parametrize("n_seq,ctx_len,q_len", [(4, 6000, 16), (3, 9000, 11), (2, 4000, 40)])
+def test_verify_blocks_over_expanded_pages(torch, n_seq, ctx_len, q_len):
+    """Blocks of new tokens over an E4M3 cache, whose pages are expanded to bf16 for them."""
+    rng = np.random.default_rng(10)
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(11)
+    with make(n_pages=n_seq * (ctx_len // 64 + 3), max_seqs=n_seq, max_tokens=512) as ctx:
+        steps = []
+        for i in range(n_seq):
+            s = ctx.seq_alloc()
+            n = ctx_len - 61 * i
+            fill(torch, ctx, s, n + q_len, gen, 576)
+            steps.append((s, n, q_len))
+        T = n_seq * q_len
+        q = bits(rng.standard_normal((T * 64, 576)).astype(np.float32))
+        for causal in (True, False):
+            got = run_batch(torch, ctx, steps, q, T, causal)
+            check_on_device(torch, ctx, steps, q, got, causal)
+
+
+def test_sharp_softmax(torch):
+    """Scores that grow along the prefix: the running maximum moves in almost every tile, for each token at its own places."""
+    rng = np.random.default_rng(12)
+    with make(e4m3=False, n_pages=400, max_seqs=20, max_tokens=512) as ctx:
+        base = ctx.seq_alloc()
+        n = 64 * 160
+        x = rng.standard_normal((n, 576)).astype(np.float32) * 0.05
+        x[:, 0] = np.linspace(0, 40, n)
+        x[:, 1] = np.linspace(40, 0, n)
+        x[:, 570] = 30 * np.sin(np.linspace(0, 60, n))
+        ctx.cache_write(0, base, 0, bits(x))
+        seqs = [ctx.seq_fork(base, n) for _ in range(16)]
+        steps = [(s, n, 1, -1, 0) for s in seqs]
+        q = np.zeros((16, 64, 576), np.float32)
+        q[:, :, 0] = rng.uniform(0, 60, (16, 64))
+        q[:, :, 1] = rng.uniform(0, 60, (16, 64))
+        q[:, :, 570] = rng.uniform(-40, 40, (16, 64))
+        q = bits(q.reshape(16 * 64, 576))
+        got = run_batch(torch, ctx, steps, q, 16, False)
+        check_on_device(torch, ctx, steps, q, got, False)

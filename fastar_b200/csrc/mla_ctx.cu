@@ -1856,13 +1856,13 @@ bool cut_block_schedule(const FstMlaCtx* c, int T, std::vector<AttnSeg>* segs_ou
 // Sequences of the plan that share their first pages.  Fills group_of[step] (-1: alone) and, per group, the number
 // of pages that all its members begin with.
 struct PrefixGroups {
-  std::vector<int> group_of, pages, tokens;
+  std::vector<int> group_of, pages, members;
 };
 void find_prefix_groups(const FstMlaCtx* c, PrefixGroups* out) {
   const int n = (int)c->pl_steps.size();
   out->group_of.assign(n, -1);
   out->pages.clear();
-  out->tokens.clear();
+  out->members.clear();
   std::vector<int> first;                         // the member each group is compared with
   std::vector<std::pair<int32_t, int>> by_page;   // (first page, step), sorted: members side by side
   for (int b = 0; b < n; ++b) {
@@ -1877,18 +1877,15 @@ void find_prefix_groups(const FstMlaCtx* c, PrefixGroups* out) {
     if (j - i >= 2) {
       const auto& t0 = c->tables[c->pl_steps[by_page[i].second].seq];
       size_t common = t0.size();
-      int toks = 0;
-      for (size_t k = i; k < j; ++k) {
-        const FstMlaSeqStep& st = c->pl_steps[by_page[k].second];
-        const auto& t = c->tables[st.seq];
+      for (size_t k = i + 1; k < j; ++k) {
+        const auto& t = c->tables[c->pl_steps[by_page[k].second].seq];
         common = std::min(common, t.size());
         for (size_t q = 0; q < common; ++q)
           if (t[q] != t0[q]) common = q;
-        toks += st.q_len;
       }
       for (size_t k = i; k < j; ++k) out->group_of[by_page[k].second] = (int)out->pages.size();
       out->pages.push_back((int)common);
-      out->tokens.push_back(toks);
+      out->members.push_back((int)(j - i));
     }
     i = j;
   }
@@ -1954,9 +1951,11 @@ int cut_epoch_schedule(const FstMlaCtx* c, int T, const PrefixGroups& pg, long l
   return n_ep;
 }
 
-// Room for n partials.  What was there stays allocated: a captured graph may still write to it.
-bool more_parts(FstMlaCtx* c, int n) {
-  if (n <= c->max_parts) return true;
+// Room for n partials, at least twice what there was (so that a batch that grows step by step does not come back each
+// time).  What was there stays allocated: a captured graph may still write to it.
+bool more_parts(FstMlaCtx* c, int want) {
+  if (want <= c->max_parts) return true;
+  const size_t n = std::max(want, 2 * c->max_parts);
   float *m = nullptr, *l = nullptr, *o = nullptr;
   const size_t H = c->d.H;
   if (cudaMalloc((void**)&m, n * H * sizeof(float)) != cudaSuccess || cudaMalloc((void**)&l, n * H * sizeof(float)) != cudaSuccess ||
@@ -1973,7 +1972,7 @@ bool more_parts(FstMlaCtx* c, int n) {
   c->d_part_m = m;
   c->d_part_l = l;
   c->d_part_o = o;
-  c->max_parts = n;
+  c->max_parts = (int)n;
   return true;
 }
 
@@ -2077,12 +2076,8 @@ int plan_schedule_part(FstMlaCtx* c, bool on_copy_stream) {
       const FstMlaSeqStep& step = c->pl_steps[b];
       if (step.q_len > 0) rows_once += step.append ? step.pos0 + step.q_len : step.pos0;
     }
-    if (!pg.pages.empty())
-      for (size_t g = 0; g < pg.pages.size(); ++g) {
-        long long members = 0;
-        for (int x : pg.group_of) members += x == (int)g;
-        rows_once = std::max(1ll, rows_once - (members - 1) * pg.pages[g] * (long long)c->cfg.page_tokens);
-      }
+    for (size_t g = 0; g < pg.pages.size(); ++g)
+      rows_once = std::max(1ll, rows_once - (pg.members[g] - 1ll) * pg.pages[g] * c->cfg.page_tokens);
     // E4M3 pages that are read often are expanded: the attention then reads bf16 pages of a scratch pool
     long long pairs = 0, page_read = (long long)c->page_bytes;
     for (int t = 0; t < T; ++t) pairs += std::max(0, kvlen[t] - kvlo[t]);
@@ -2091,7 +2086,7 @@ int plan_schedule_part(FstMlaCtx* c, bool on_copy_stream) {
       S.n_expand = (int)xpages.size();
       page_read = (long long)c->cfg.page_tokens * c->d.row * (long long)sizeof(bf16);
     }
-    const bool stays_in_l2 = rows_once / c->cfg.page_tokens * page_read <= L2_ROWS_BYTES;
+    const bool stays_in_l2 = rows_once * (page_read / c->cfg.page_tokens) <= L2_ROWS_BYTES;
     S.by_blocks = k == 0 && c->block_schedule && cut_block_schedule(c, T, &segs, &cta_seg, &tok_part, &kv_rows);
     S.n_epochs = 1;
     if (!S.by_blocks) {

@@ -378,12 +378,16 @@ class MlaContext:
 
     def cache_append_device(self, lid: int, d_rows: int) -> None:
         """Device rows bf16 [T, row] become the cache rows of the current plan's new tokens."""
-        self._check(self.lib.fst_cuda_mla_cache_append_device(self._h, lid, C.c_void_p(d_rows)))
+        rc = self.lib.fst_cuda_mla_cache_append_device(self._h, lid, d_rows)
+        if rc:
+            self._check(rc)
 
     def cache_read_device(self, lid: int, ranges, d_rows: int) -> None:
         """ranges: (seq, pos0, n) tuples, or seq_steps() of them; their rows as bf16, one range behind the other."""
         arr = seq_steps(ranges)
-        self._check(self.lib.fst_cuda_mla_cache_read_device(self._h, lid, arr, len(arr), C.c_void_p(d_rows)))
+        rc = self.lib.fst_cuda_mla_cache_read_device(self._h, lid, arr, len(arr), d_rows)
+        if rc:
+            self._check(rc)
 
     def pool_read(self, lid: int) -> np.ndarray:
         """A layer's pool as it is held: bf16 rows [n_pages * page_tokens, row], or (E4M3) bytes [n_pages, page bytes]."""
@@ -511,7 +515,9 @@ class MlaContext:
 
     def attention_device(self, lid: int, d_q_eff: int, d_o_lat: int) -> None:
         """attention_only() on device buffers: bf16 [T * heads, d_qk] -> bf16 [T * heads, d_v]."""
-        self._check(self.lib.fst_cuda_mla_attention_device(self._h, lid, C.c_void_p(d_q_eff), C.c_void_p(d_o_lat)))
+        rc = self.lib.fst_cuda_mla_attention_device(self._h, lid, d_q_eff, d_o_lat)
+        if rc:
+            self._check(rc)
 
     def get_stage(self, stage: int) -> np.ndarray:
         T, H, d, c = self.plan_tokens(), self.cfg.n_heads, self.dims, self.cfg

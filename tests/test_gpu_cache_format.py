@@ -386,6 +386,26 @@ def test_window(torch):
                             mla.default_scale(ctx.cfg), None, [0], 64, False)
 
 
+def test_window_over_a_prompt(torch):
+    """Many rows with a sliding window: pages are expanded, from the first one that some token sees."""
+    rng = np.random.default_rng(14)
+    with make(n_pages=20, max_tokens=400) as ctx:
+        s, t = ctx.seq_alloc(), ctx.seq_alloc()
+        values = []
+        for q, n in ((s, 400), (t, 150)):
+            ctx.cache_write(0, q, 0, bits(rng.standard_normal((n, 576)).astype(np.float32)))
+            values.append(f32(ctx.cache_read(0, q, 0, n)).astype(np.float64))
+        steps = [(s, 150, 250, -1, 1, 70), (t, 0, 150, -1, 1, 33)]
+        q = bits(rng.standard_normal((400 * 64, 576)).astype(np.float32))
+        d_q, d_o = dev(torch, q), dev(torch, np.zeros((400 * 64, 512), np.uint16))
+        ctx.plan(steps, causal=True)
+        ctx.attention_device(0, d_q.data_ptr(), d_o.data_ptr())
+        ctx.sync()
+        keys = [v[max(0, p + i + 1 - w):p + i + 1] for v, (_, p, n, _, _, w) in zip(values, steps) for i in range(n)]
+        check_attention(host(d_o).reshape(400, 64, 512), f32(q).astype(np.float64).reshape(400, 64, 576), keys, 512,
+                        mla.default_scale(ctx.cfg), None, [0] * 400, 64, False)
+
+
 @pytest.mark.parametrize("preset", [mla.PRESET_BASELINE, mla.PRESET_FASTAR_V4])
 def test_layer_calls(torch, preset):
     """Layer calls over an E4M3 cache: the rows they append are the quantised STAGE_KV rows, and a bf16 context

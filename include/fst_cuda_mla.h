@@ -120,7 +120,7 @@ typedef struct FstMlaSeqStep {
 /* Intermediate buffers of the last run, the stage list of FST_MLA_TRACE
  * (src/fst_engine.cpp:3396-3407, 3521-3532, 3685-3695, 3841-3851). */
 #define FST_MLA_STAGE_QC 0    /* [T, q_lora]      after wq_a + q_norm */
-#define FST_MLA_STAGE_KV 1    /* [T, row]         new cache rows (normed latent, rotated k_pe) */
+#define FST_MLA_STAGE_KV 1    /* [T, row]         new cache rows (normed latent, rotated k_pe; before an E4M3 cache rounds them) */
 #define FST_MLA_STAGE_QEFF 2  /* [T*H, d_qk]      query in latent space, RoPE applied */
 #define FST_MLA_STAGE_OLAT 3  /* [T*H, d_v]       attention output (V4: after inverse RoPE) */
 #define FST_MLA_STAGE_LOW 4   /* [T, 8192]        after O-proj a */
@@ -319,7 +319,8 @@ int fst_cuda_mla_forward(FstMlaCtx* ctx, int lid, const uint16_t* h_in, uint16_t
 int fst_cuda_mla_attention_only(FstMlaCtx* ctx, int lid, const uint16_t* q_eff, uint16_t* o_lat);
 /* The same with device buffers: d_q_eff bf16 [T*H, d_qk] -> d_o_lat bf16 [T*H, d_v], both 16-byte aligned (not
  * the same buffer).  Enqueued on the context's stream, no synchronisation; may be captured into a graph, which
- * is valid until the next plan.  Layer weights are needed in the V4 form only (the sink logits). */
+ * is valid until the next plan.  Layer weights are needed in the V4 form only (the sink logits).  A NaN in a cached row
+ * reaches every token whose 64-row tile holds the row, also one that does not see it (probability 0 times NaN). */
 int fst_cuda_mla_attention_device(FstMlaCtx* ctx, int lid, const void* d_q_eff, void* d_o_lat);
 /* Split-KV across GPUs: run the layer up to the merged per-GPU partial.  d_partial is device
  * fp32 [T*H, 2 + d_v] holding (max, sum, un-normalised O) per query row. */

@@ -106,7 +106,8 @@ __device__ __forceinline__ __nv_bfloat162 bf162_of_bits(uint32_t bits16) {
 }
 // The same where 2^k is a normal fp16 number (scale bytes 113 .. 142): codes to fp16, a multiplication that widens to
 // fp32, two packed to bf16; every step exact.  On the integer pipe a pair of codes costs half of what the
-// bit moves above do (16 x 2048 codes per warp of four: 1630 cycles instead of 2110, loads and stores included).
+// bit moves above do (64 x 512 codes by four warps of an otherwise idle SM: 1630 cycles instead of 2110, shared-memory
+// loads and stores included).
 // scale_f16: the bits of 2^k.
 __device__ __forceinline__ uint2 e4m3_to_bf16x4_near(uint32_t w, uint32_t scale_f16) {
   float f0, f1, f2, f3;

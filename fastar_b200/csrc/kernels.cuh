@@ -238,7 +238,7 @@ void set_last_error(const char* msg);
 // every ratio-th position the pooled / normed / tail-rotated / E4M3-round-tripped row, written to
 // the compressed-row pages.
 struct CompressTok {
-  long long dst;   // element offset of the compressed row this token emits in the pool, or -1
+  long long dst;   // element offset (E4M3 pools: the pool row) of the compressed row this token emits, or -1
   int32_t pos;     // position of the token in its sequence
   int32_t pad;
 };
@@ -254,7 +254,7 @@ struct CompressArgs {
   const CompressTok* toks;   // [T]
   const CompressStep* steps; // [n_steps]
   float* state;              // [slots][2][rows, width] window state (values, then scores)
-  bf16* pool;
+  PoolView pool;
   int n_steps, ratio, width, kv_lora, rope;
 };
 void launch_compress(const CompressArgs& a, cudaStream_t st);

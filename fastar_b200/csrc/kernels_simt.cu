@@ -1120,7 +1120,23 @@ __global__ void __launch_bounds__(512) k_compress(CompressArgs a) {
         const float scale = ldexpf(1.0f, (int)ceilf(log2f(amax / 448.0f)));
         v = e4m3_roundtrip(fminf(448.0f, fmaxf(-448.0f, v / scale))) * scale;
       }
-      if (tk.dst >= 0) a.pool[tk.dst + j] = f2bf(v);
+      if (!a.pool.e4m3 && tk.dst >= 0) reinterpret_cast<bf16*>(a.pool.base)[tk.dst + j] = f2bf(v);
+    }
+    if (a.pool.e4m3 && tk.dst >= 0) {
+      // The values are E4M3 times a power of two already.  Quantised again, with a scale that is the least for what the
+      // rounding left (never a larger one), each is held exactly.
+      __syncthreads();
+      if (j < hd) s_out[j] = v;
+      __syncthreads();
+      for (int u0 = 0; u0 < hd / 8; u0 += blockDim.x) {
+        const int u = u0 + threadIdx.x;
+        const bool has = u < hd / 8;
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = has ? s_out[u * 8 + e] : 0.0f;
+        store_unit(a.pool, tk.dst, u, pack8(x), has);
+      }
+      __syncthreads();
     }
     // window rotation, ratio 4 (3302-3317): the window just processed becomes the previous one
     if (ratio == 4) {

@@ -627,7 +627,7 @@ int run_front(FstMlaCtx* c, int lid, const bf16* h_in) {
     if ((rc = run_gemm(c, plain_gemm(h_in, w.w_cmp_proj, c->d_cproj, T, 2 * width, d.hidden)))) return rc;
     CompressArgs ca;
     ca.proj = c->d_cproj; ca.ape = w.cmp_ape; ca.norm = w.cmp_norm; ca.lut = S.d_lut_cmp; ca.toks = S.d_ctoks;
-    ca.steps = S.d_csteps; ca.state = w.cmp_state; ca.pool = c->pools[lid]; ca.n_steps = S.n_csteps;
+    ca.steps = S.d_csteps; ca.state = w.cmp_state; ca.pool = view_of(c, lid); ca.n_steps = S.n_csteps;
     ca.ratio = w.cmp_ratio; ca.width = width; ca.kv_lora = d.kv_lora; ca.rope = d.rope;
     launch_compress(ca, c->stream);
     c->launches += 1;
@@ -1027,7 +1027,6 @@ int fst_cuda_mla_set_layer_compressor(FstMlaCtx* c, int lid, const FstMlaCompres
   const int ratio = w ? w->ratio : 0;
   if (ratio != 0 && ratio != 4 && ratio != 128) return fail(FST_MLA_ERR_ARG, "compress ratio %d (0, 4 or 128)", ratio);
   if (ratio && (!w->wkv || !w->wgate || !w->ape || !w->norm)) return fail(FST_MLA_ERR_ARG, "a compressor tensor is NULL");
-  if (ratio && c->e4m3) return fail(FST_MLA_ERR_STATE, "the KV compressor writes bf16 rows: not with an E4M3 cache");
   for (int s = 0; s < c->cfg.max_seqs; ++s)
     if (c->live[s] && c->lens[s] > 0)
       return fail(FST_MLA_ERR_STATE, "set the compressors before any sequence holds rows");
@@ -1093,6 +1092,24 @@ int fst_cuda_mla_cmp_read(FstMlaCtx* c, int lid, int32_t seq, uint16_t* rows, in
   if (cap < n) return fail(FST_MLA_ERR_ARG, "%d compressed rows, room for %d", n, cap);
   CU(cudaSetDevice(c->cfg.device));
   const int pt = c->cfg.page_tokens, row = c->d.row;
+  if (c->e4m3) {
+    for (int done = 0; done < n;) {
+      RowRuns r;
+      int k = 0, turn = 0;
+      while (done + turn < n && turn < ROWS_TMP && k < RowRuns::CAP) {
+        const int at = done + turn, run = std::min({n - at, pt - at % pt, ROWS_TMP - turn});
+        r.run[k++] = RowRun{c->comp_tables[seq][at / pt] * pt + at % pt, turn, run};
+        turn += run;
+      }
+      c->status_by_kernel = false;
+      CU(launch_rows_runs(view_of(c, lid), c->d_rows_tmp, r.run, nullptr, k, std::min(pt, turn), false, c->stream));
+      c->launches += 1;
+      CU(cudaMemcpyAsync(rows + (size_t)done * row, c->d_rows_tmp, (size_t)turn * row * 2, cudaMemcpyDeviceToHost, c->stream));
+      done += turn;
+    }
+    CU(cudaStreamSynchronize(c->stream));
+    return FST_MLA_OK;
+  }
   for (int r = 0; r < n; ++r) {
     const bf16* src = c->pools[lid] + ((long long)c->comp_tables[seq][r / pt] * pt + r % pt) * row;
     CU(cudaMemcpyAsync(rows + (size_t)r * row, src, (size_t)row * 2, cudaMemcpyDeviceToHost, c->stream));
@@ -1410,7 +1427,6 @@ int fst_cuda_mla_set_cache_format(FstMlaCtx* c, int32_t format) {
       return fail(FST_MLA_ERR_ARG, "an E4M3 cache needs latent and rope widths that are multiples of 8");
     if ((long long)c->cfg.n_pages * c->cfg.page_tokens >= (1ll << 31))
       return fail(FST_MLA_ERR_ARG, "an E4M3 cache has fewer than 2^31 rows per layer");
-    if (c->has_cmp) return fail(FST_MLA_ERR_STATE, "the KV compressor writes bf16 rows: not with an E4M3 cache");
   }
   for (int s = 0; s < c->cfg.max_seqs; ++s)
     if (c->live[s] && c->lens[s] > 0)
@@ -1682,7 +1698,7 @@ int plan_tokens_part(FstMlaCtx* c, const FstMlaSeqStep* steps, int32_t n_seqs, i
         if (st.append && (pos + 1) % ratio == 0) {
           // compressed row number (pos + 1) / ratio - 1, rotated at position pos + 1 - ratio (3252-3254)
           const int cr = (pos + 1) / ratio - 1;
-          ctoks[tt].dst = ((long long)c->comp_tables[st.seq][cr / pt] * pt + cr % pt) * d.row;
+          ctoks[tt].dst = ((long long)c->comp_tables[st.seq][cr / pt] * pt + cr % pt) * (c->e4m3 ? 1 : d.row);
           memcpy(&lut_cmp[(size_t)tt * d.rope], lut_row_cached(c, kind, pos + 1 - ratio), (size_t)d.rope * sizeof(float));
         }
       }

@@ -119,7 +119,7 @@ class FSTEngine {
   // The KV compressor runs for layers that carry its weights (the reference gates it behind the
   // FST_COMPRESSOR environment variable, 3565): off by default here too; call before preload_all_layers.
   void enable_compressor(bool on) { use_compressor_ = on; }
-  // What the cache holds, FST_MLA_CACHE_BF16 (as the reference) or _E4M3; before any row is in it, and not with the compressor.
+  // What the cache holds, FST_MLA_CACHE_BF16 (as the reference) or _E4M3; before any row is in it.
   void set_cache_format(int format);
   // Sliding window of the draft model's attention (draft_cfg_.window_size, 2534-2576): process_mla
   // attends to the last `window` rows only; 0 switches it off.

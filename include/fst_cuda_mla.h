@@ -247,9 +247,10 @@ int fst_cuda_mla_cache_read(FstMlaCtx* ctx, int lid, int32_t seq, int32_t pos0, 
  * whole group NaN.  Every call that writes rows quantises them (the layer calls, append_rows, cache_write,
  * cache_append_device), every call that reads them gives the bf16 values they stand for (cache_read,
  * cache_read_device), and the attention multiplies exactly these values.  A layer call's own new rows are
- * attended to in their quantised form.  Not with a KV compressor (its rows are bf16), and
- * fst_cuda_mla_row_offset has no answer then.  FST_MLA_ERR_STATE if a sequence holds rows or a layer has
- * a compressor, FST_MLA_ERR_ARG if latent or rope width is no multiple of 8. */
+ * attended to in their quantised form; rows that the KV compressor emits are E4M3 values already and are held
+ * exactly.  fst_cuda_mla_row_offset has no answer then.  The old pools are freed: a graph captured before is not to
+ * be replayed.  FST_MLA_ERR_STATE if a sequence holds rows, FST_MLA_ERR_ARG if latent or rope width is no
+ * multiple of 8. */
 int fst_cuda_mla_set_cache_format(FstMlaCtx* ctx, int32_t format);
 /* Bytes of a page of page_tokens rows in one layer's pool, in the present format. */
 int fst_cuda_mla_cache_page_bytes(FstMlaCtx* ctx, int64_t* bytes_out);

@@ -440,6 +440,44 @@ def test_layer_calls(torch, preset):
         assert ctx.seq_len(seqs[0]) == pos[0] + 2
 
 
+def test_compressed_layers(torch):
+    """A ratio-4 and a ratio-128 layer over an E4M3 cache: the compressed rows are those of a bf16 context bit for bit (they are
+    E4M3 values already), and the attention over raw and compressed rows is what the bf16 context gives when it
+    holds the quantised raw rows."""
+    rng = np.random.default_rng(15)
+    kw = dict(hidden=256, q_lora=128, o_lora=128, n_layers=2, n_pages=60, max_seqs=2, max_tokens=160)
+    with make(mla.PRESET_FASTAR_V4, e4m3=False, **kw) as ctx, make(mla.PRESET_FASTAR_V4, e4m3=False, **kw) as plain:
+        for c in (ctx, plain):
+            wr = np.random.default_rng(16)
+            for lid, ratio in enumerate((4, 128)):
+                c.set_layer_weights(lid, synth.weights_to_bits(synth.layer_weights_f32(c.cfg, lid, 0)))
+                c.set_layer_rope(lid, True)
+                width = 1024 if ratio == 4 else 512
+                m = [bits(wr.standard_normal((width, 256)).astype(np.float32) * 0.1) for _ in range(2)]
+                c.set_layer_compressor(lid, ratio, *m, wr.standard_normal((ratio, width)).astype(np.float32),
+                                       bits((1 + 0.1 * wr.standard_normal(512)).astype(np.float32)))
+        ctx.set_cache_format(mla.CACHE_E4M3)
+        seqs = [ctx.seq_alloc(), ctx.seq_alloc()]
+        assert [plain.seq_alloc(), plain.seq_alloc()] == seqs
+        pos = [0, 0]
+        for q_lens, causal in (((150, 10), True), ((130, 20), True), ((1, 1), False), ((6, 6), True)):
+            h = bits(rng.standard_normal((sum(q_lens), 256)).astype(np.float32))
+            for lid in range(2):
+                ctx.forward(lid, h, seqs, pos, list(q_lens), causal=causal)
+                q_eff, o_lat = ctx.get_stage(mla.STAGE_QEFF), ctx.get_stage(mla.STAGE_OLAT)
+                plain.forward(lid, h, seqs, pos, list(q_lens), causal=causal)
+                for s, p, n in zip(seqs, pos, q_lens):
+                    a, b = ctx.cmp_read(lid, s), plain.cmp_read(lid, s)
+                    assert a.shape == ((p + n) // (4, 128)[lid], 512) and np.array_equal(a, b)
+                    plain.cache_write(lid, s, p, ctx.cache_read(lid, s, p, n))
+                plain.plan([(s, p, n) for s, p, n in zip(seqs, pos, q_lens)], causal=causal)
+                assert np.array_equal(plain.attention_only(lid, q_eff), o_lat)
+            pos = [p + n for p, n in zip(pos, q_lens)]
+        ctx.seq_truncate(seqs[0], 0)
+        ctx.forward(0, h[:6], [seqs[0]], [0], [6], causal=True)
+        assert ctx.cmp_read(0, seqs[0]).shape == (1, 512)
+
+
 def test_split_over_two_slices(torch):
     """Partials of two contexts, each with a slice of the rows, merged: what one context with all rows gives."""
     rng = np.random.default_rng(10)
@@ -568,11 +606,5 @@ def test_refusals(torch):
         s = ctx.seq_alloc()
         ctx.plan([(s, 0, 1)])
         refused(mla.ERR_STATE, ctx.attention_device, 0, p, p)  # no weights: no sink logits
-        z = lambda *sh: np.zeros(sh, np.uint16)  # noqa: E731
-        ctx.seq_free(s)
-        refused(mla.ERR_STATE, ctx.set_layer_compressor, 0, 4, z(1024, 64), z(1024, 64), np.zeros((4, 1024), np.float32), z(512))
-        ctx.set_cache_format(mla.CACHE_BF16)
-        ctx.set_layer_compressor(0, 4, z(1024, 64), z(1024, 64), np.zeros((4, 1024), np.float32), z(512))
-        refused(mla.ERR_STATE, ctx.set_cache_format, mla.CACHE_E4M3)
     with make(mla.PRESET_FASTAR_V4, e4m3=False, kv_lora=64, qk_rope=12, n_heads=8) as ctx:  # 52 latent values
         refused(mla.ERR_ARG, ctx.set_cache_format, mla.CACHE_E4M3)

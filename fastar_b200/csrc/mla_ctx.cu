@@ -116,6 +116,12 @@ constexpr long long L2_ROWS_BYTES = 64ll << 20;
 // 62 000 rows 924 / 1128; E4M3, 6 users over 130 000 rows 183 / 178.  Epochs of 24 MiB: 24 users 520; of 80 MiB:
 // 496, and 64 users over 62 000 rows (71 MB, then one epoch) 718 against 601.
 constexpr int EPOCH_READS = 8;
+// Users of one prefix, a new token each, take the schedule of blocks (a lane per user) where whole groups of lanes use this
+// much of the SMs.  With / without it, us, bf16: 24 users over 130 000 rows 458 / 485, 8 users 169 / 204, 4 users 92 / 101, 16
+// users 316 / 336, 140 users over 62 000 rows (94 %) 1273 / 1290, 148 users over 1500 rows 47.6 / 58, 24 users over
+// 4000 32.5 / 35.3, 8 users over 16 384 40.6 / 39.8; at 91 % (45 and 67 users over 62 000 rows) 439 / 439 and 647 / 647, at 81 %
+// (40 users) 441 / 389, at 68 % (100 users) 1309 / 925.
+constexpr int LANES_PERCENT = 92;
 constexpr long long EPOCH_BYTES = 48ll << 20;
 constexpr int MAX_EPOCHS = 8;
 // An E4M3 page that a call reads this many times is worth turning into bf16 once for all of them (the kernel that
@@ -1809,18 +1815,18 @@ void cut_schedule(const FstMlaCtx* c, const std::vector<TileStream>& streams, in
 // the token schedule cuts tiles; lane i of a group walks its group's run for token i of each
 // sequence, so the G lanes read the same page at about the same time and it crosses the HBM
 // interface once.  Returns false (nothing written) when the call is not of that shape.
+// one_group: all T tokens of the plan are users of one prefix, a single block of G = T whose lanes go on in their own tables.
 bool cut_block_schedule(const FstMlaCtx* c, int T, std::vector<AttnSeg>* segs_out, std::vector<int32_t>* cta_seg_out,
-                        std::vector<int32_t>* tok_part_out, long long* kv_rows_out) {
+                        std::vector<int32_t>* tok_part_out, long long* kv_rows_out, bool one_group = false) {
   const int unit = 64;
   if (c->cfg.page_tokens != unit) return false;
-  int G = 0, n_seq = 0;
+  int G = one_group ? T : 0;
   for (const FstMlaSeqStep& st : c->pl_steps) {
-    if (st.q_len == 0) continue;
+    if (st.q_len == 0 || one_group) continue;
     if (G && st.q_len != G) return false;
     G = st.q_len;
-    ++n_seq;
   }
-  if (G < 4 || G > c->n_sm) return false;
+  if ((G < 4 && !one_group) || G > c->n_sm) return false;
   for (int t = 0; t < T; ++t)
     if (c->pl_kvlo[t] != 0) return false;  // sliding windows keep the token schedule
   const int n_groups = c->n_sm / G;
@@ -2106,11 +2112,16 @@ int plan_schedule_part(FstMlaCtx* c, bool on_copy_stream) {
     S.by_blocks = k == 0 && c->block_schedule && cut_block_schedule(c, T, &segs, &cta_seg, &tok_part, &kv_rows);
     S.n_epochs = 1;
     if (!S.by_blocks) {
-      if (!pg.pages.empty() && !stays_in_l2 && pairs >= EPOCH_READS * rows_once) {
+      // users of one prefix whose number fills the SMs in whole groups: lanes side by side, as for the tokens of a block
+      const bool lanes = pg.pages.size() == 1 && pg.members[0] == T && T <= c->n_sm &&
+                         c->n_sm / T * T * 100 >= LANES_PERCENT * c->n_sm;
+      if (lanes && cut_block_schedule(c, T, &segs, &cta_seg, &tok_part, &kv_rows, true)) {
+        S.by_blocks = true;
+      } else if (!pg.pages.empty() && !stays_in_l2 && pairs >= EPOCH_READS * rows_once) {
         const int n = cut_epoch_schedule(c, T, pg, page_read, &segs, &cta_seg, &tok_part, &kv_rows);
         if (n > 0 && (int)segs.size() <= c->segs_cap && more_parts(c, (int)segs.size())) S.n_epochs = n;
       }
-      if (S.n_epochs == 1) cut_schedule(c, streams, T, &segs, &cta_seg, &tok_part, &kv_rows);
+      if (S.n_epochs == 1 && !S.by_blocks) cut_schedule(c, streams, T, &segs, &cta_seg, &tok_part, &kv_rows);
     }
     if ((int)segs.size() > c->segs_cap || (int)segs.size() > c->max_parts)
       return fail(FST_MLA_ERR_CAPACITY, "split schedule overflow");

@@ -292,9 +292,10 @@ int fst_cuda_mla_set_fused_merge(FstMlaCtx* ctx, int32_t on);
  * Default: on. */
 int fst_cuda_mla_set_block_schedule(FstMlaCtx* ctx, int32_t on);
 /* Calls in which sequences share pages (fst_cuda_mla_seq_fork): the plan counts what the batch reads by distinct
- * pages.  A prefix that stays in L2 is walked token by token with the tiles kept there; a longer one in epochs,
- * stretches of pages that do stay there and that all thread blocks walk at about the same time, so that each
- * page comes from HBM once.  on = 0: scheduled as if nothing were shared.  Results do not depend on it beyond the order
+ * pages.  Users of one prefix read its pages side by side, as the tokens of a block do, where their number suits the
+ * device; else a prefix that stays in L2 is walked token by token with the tiles kept there, a longer one in epochs,
+ * stretches of pages that do stay there and that all thread blocks walk at about the same time.  Each page then
+ * comes from HBM once.  on = 0: scheduled as if nothing were shared.  Results do not depend on it beyond the order
  * in which a token's parts are added.  Default: on. */
 int fst_cuda_mla_set_shared_prefix(FstMlaCtx* ctx, int32_t on);
 /* Sliding window that fst_cuda_mla_forward applies to every sequence of its calls (0: none). */

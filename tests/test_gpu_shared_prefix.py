@@ -438,6 +438,9 @@ LONG = [
     (6401, 24, 70, 1, 0),       # a prefix that ends inside a page
     (3000, 20, 90, 3, 1),       # blocks of new tokens on a shared prefix
     (20000, 8, 300, 1, 0),
+    (700, 148, 400, 1, 0),      # a lane for every SM; own rows longer than the prefix for some
+    (130, 74, 130, 1, 0),
+    (5000, 2, 900, 1, 0),
 ]
 
 

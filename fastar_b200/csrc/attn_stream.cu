@@ -319,6 +319,15 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
+// Arrives at a barrier once `value` is there: the comparison (whose outcome only picks a pause) waits for it.
+__device__ __forceinline__ void arrive_behind(uint64_t* bar, uint32_t value) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.eq.u32 p, %1, 0x12345678;\n\t"
+      "@p nanosleep.u32 1;\n\t"
+      "mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(tc::smem_u32(bar)), "r"(value)
+      : "memory");
+}
 // A barrier wait of a whole warp: all lanes go on, or none.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* d_status, int code) {
   return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_flag, d_status, code));
@@ -604,9 +613,12 @@ k_attn_stream(const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ 
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(&mi->full_t[g & 3][i]);
         };
-        auto stage_read = [&]() {
+        // The stage's copy may be overwritten once what was loaded from it has ARRIVED in registers: a load still on its
+        // way is not held by an arrival behind it (built that way, rows of the next page came in).  `last` comes from the
+        // last load; a warp's loads return in order.
+        auto stage_read = [&](uint32_t last) {
           __syncwarp();
-          if (lane == 0) tc::mbar_arrive(&mi->st_free[n & 1]);
+          if (lane == 0) arrive_behind(&mi->st_free[n & 1], last);
         };
         auto second_piece = [&]() { return warp_wait(&mi->st_full[n & 1][1], par, abort_flag, p.d_status, ST_DEQ_TIMEOUT); };
         if (!wide) {
@@ -637,10 +649,10 @@ k_attn_stream(const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ 
             const uint4 w6 = lds128(codes + 6 * E8_GROUP);
             uint4 w7 = w6;
             if (NCH == 9) w7 = lds128(codes + 7 * E8_GROUP);
+            stage_read(w7.w);
             turn(6, w6);
             if (NCH == 9) turn(7, w7);
           }
-          stage_read();
           if (!frame_free()) break;
 #pragma unroll
           for (int c = 0; c < 3; ++c) store(c, o[c]);
@@ -663,9 +675,10 @@ k_attn_stream(const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ 
             store(c, o);
             if (c == 2 || c == 5) arrive(c / 3);
           }
-          store_rope(0, load_rope(0));
-          store_rope(1, load_rope(1));
-          stage_read();
+          const uint4 ra = load_rope(0), rb = load_rope(1);
+          store_rope(0, ra);
+          store_rope(1, rb);
+          stage_read(rb.w);
         }
         // the next page is asked for before this tile's last arrival: the answer takes a few hundred cycles
         ready = tc::mbar_test_wait(&mi->st_full[(n + 1) & 1][0], ((n + 1) >> 1) & 1);

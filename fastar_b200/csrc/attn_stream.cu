@@ -379,7 +379,7 @@ __device__ __forceinline__ bool qk_chunks(StreamMisc* mi, int g, uint32_t d, uin
 // store the next tile (72 KB, from registers), 2000 for its QK MMAs (which share the tensor pipe with the
 // other tile's SV), 1400 for the softmax and 1600 for the SV MMAs; a tile every 3500 cycles, of which the pipe is
 // busy 2176 and HBM would need 1600.  With the dequantisation behind the wait for the frame instead of in front
-// of it the same tile took 4300 (64 users x 1024-8192 rows 94 us, now 82), by four warps instead of eight 4850
+// of it the same tile took 4300 (64 users x 1024-8192 rows 94 us, now 87), by four warps instead of eight 4850
 // (117), with a branch on the scale per 16 codes 7000 (133).  Chunks 0-3 released after the first half of the SV
 // MMAs: 88.
 template <int NCH, bool DIRECT, bool WHOLE, bool FLAT, bool E8>

@@ -402,6 +402,14 @@ PoolView view_of(const FstMlaCtx* c, int lid) {
   return pool_view(c->pools[lid], c->e4m3, c->d.row, c->d.rope, c->cfg.page_tokens);
 }
 
+// Pages are copied when the tables change, not when a graph is replayed.
+int no_capture(FstMlaCtx* c, const char* what) {
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  CU(cudaStreamIsCapturing(c->stream, &cap));
+  if (cap != cudaStreamCaptureStatusNone) return fail(FST_MLA_ERR_STATE, "%s copies a page: not while its stream is captured", what);
+  return FST_MLA_OK;
+}
+
 // Copy on write: pages of rows [pos0, pos0 + n) that other sequences hold too become this sequence's own.  (A
 // shared page is full of rows that all its holders see: who is truncated into one has had it replaced.)
 int own_rows(FstMlaCtx* c, int32_t seq, int32_t pos0, int32_t n) {
@@ -414,6 +422,10 @@ int own_rows(FstMlaCtx* c, int32_t seq, int32_t pos0, int32_t n) {
   if (need > c->free_pages.size())
     return fail(FST_MLA_ERR_PAGES, "page pool exhausted: sequence %d writes into %zu shared pages, %zu free", seq, need,
                 c->free_pages.size());
+  if (need > 0) {
+    const int rc = no_capture(c, "a write into a shared page");
+    if (rc) return rc;
+  }
   for (int p = p0; p <= p1; ++p) {
     const int32_t old = t[p];
     if (c->page_ref[old] <= 1) continue;
@@ -1165,6 +1177,8 @@ int fst_cuda_mla_seq_truncate(FstMlaCtx* c, int32_t seq, int32_t n_tokens) {
     size_t back = c->free_pages.size();
     for (size_t p = keep; p < t.size(); ++p) back += c->page_ref[t[p]] == 1;
     if (back == 0) return fail(FST_MLA_ERR_PAGES, "page pool exhausted: row %d lies in a shared page", n_tokens);
+    const int rc = no_capture(c, "a truncation inside a shared page");
+    if (rc) return rc;
   }
   // zero the dropped rows in every layer, as the reference rollback does (6132-6147); rows of shared pages are the others'
   const int n_drop = c->lens[seq] - n_tokens;
@@ -1244,6 +1258,10 @@ int fst_cuda_mla_seq_fork(FstMlaCtx* c, int32_t src, int32_t n_tokens, int32_t* 
   if (rest && c->free_pages.empty())
     return fail(FST_MLA_ERR_PAGES, "page pool exhausted: the fork's last page needs a copy");
   CU(cudaSetDevice(c->cfg.device));
+  if (rest) {
+    const int rc = no_capture(c, "the fork");
+    if (rc) return rc;
+  }
   try {
     std::vector<int32_t> table(c->tables[src].begin(), c->tables[src].begin() + whole);
     table.reserve(whole + 1);

@@ -217,7 +217,9 @@ int fst_cuda_mla_seq_free(FstMlaCtx* ctx, int32_t seq);
  * two are sequences of their own: each appends, is truncated and freed by itself, a page returns to the
  * pool with its last holder, a call that writes into a shared page (cache_write, a plan step with append = 1 over
  * rows that are there) gets copies of the pages it touches first, and a truncation that ends inside a shared page
- * takes a copy of what stays.  FST_MLA_ERR_PAGES when no page is left for such a copy (nothing has changed then).
+ * takes a copy of what stays.  FST_MLA_ERR_PAGES when no page is left for such a copy, FST_MLA_ERR_STATE where one
+ * would be made while the stream is captured (nothing has changed then).  The current plan ends, as with a truncation, and
+ * graphs captured under it: their new rows may lie in what are shared pages now.
  * A plan that holds sequences with the same first pages reads these once for all, see
  * fst_cuda_mla_set_shared_prefix.  Not in contexts with a KV compressor (FST_MLA_ERR_STATE). */
 int fst_cuda_mla_seq_fork(FstMlaCtx* ctx, int32_t src, int32_t n_tokens, int32_t* seq_out);

@@ -320,6 +320,37 @@ def test_more_table_entries_than_pages(torch):
                         [0] * 64, 64, False)
 
 
+def test_no_page_copies_in_a_capture(torch):
+    """A fork, a write or a truncation that would copy a page is refused while the stream is captured, and works behind it."""
+    rng = np.random.default_rng(7)
+    with make(e4m3=False, n_pages=12, max_seqs=3) as ctx:
+        st = torch.cuda.Stream()
+        ctx.set_stream(st.cuda_stream)
+        s = ctx.seq_alloc()
+        rows = rows_of(rng, 150)
+        ctx.cache_write(0, s, 0, rows)
+        t = ctx.seq_fork(s, 128)
+        free = ctx.free_pages()
+        ctx.sync()
+        buf = dev(torch, np.zeros((128, 576), np.uint16))
+        ctx.cache_read_device(0, [(t, 0, 128)], buf.data_ptr())  # attributes are set outside the capture
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            refused(mla.ERR_STATE, ctx.seq_fork, s, 150)
+            refused(mla.ERR_STATE, ctx.seq_truncate, t, 100)
+            ctx.cache_read_device(0, [(t, 0, 128)], buf.data_ptr())
+        assert ctx.free_pages() == free and ctx.seq_len(t) == 128
+        buf.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(host(buf), rows[:128])
+        u = ctx.seq_fork(s, 150)
+        ctx.seq_truncate(t, 100)
+        assert np.array_equal(ctx.cache_read(0, u, 0, 150), rows) and np.array_equal(ctx.cache_read(0, t, 0, 100), rows[:100])
+
+
 def test_refusals(torch):
     with make(e4m3=False, n_pages=3, max_seqs=3) as ctx:
         s = ctx.seq_alloc()

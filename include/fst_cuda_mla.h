@@ -323,8 +323,8 @@ int fst_cuda_mla_forward(FstMlaCtx* ctx, int lid, const uint16_t* h_in, uint16_t
 int fst_cuda_mla_attention_only(FstMlaCtx* ctx, int lid, const uint16_t* q_eff, uint16_t* o_lat);
 /* The same with device buffers: d_q_eff bf16 [T*H, d_qk] -> d_o_lat bf16 [T*H, d_v], both 16-byte aligned (not
  * the same buffer).  Enqueued on the context's stream, no synchronisation; may be captured into a graph, which
- * is valid until the next plan.  Layer weights are needed in the V4 form only (the sink logits).  A NaN in a cached row
- * reaches every token whose 64-row tile holds the row, also one that does not see it (probability 0 times NaN). */
+ * is valid until the next plan.  Layer weights are needed in the V4 form only (the sink logits).  A NaN or an
+ * infinity in a cached row reaches the tokens that see the row and no others. */
 int fst_cuda_mla_attention_device(FstMlaCtx* ctx, int lid, const void* d_q_eff, void* d_o_lat);
 /* Split-KV across GPUs: run the layer up to the merged per-GPU partial.  d_partial is device
  * fp32 [T*H, 2 + d_v] holding (max, sum, un-normalised O) per query row. */

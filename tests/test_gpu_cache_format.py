@@ -356,6 +356,51 @@ def test_scales_of_every_size(torch, preset, factor):
         assert np.isfinite(outs[0][64:]).all() and np.isnan(outs[0][:64]).any() == math.isnan(factor)
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -3.3e38])
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("preset", [mla.PRESET_BASELINE, mla.PRESET_FASTAR_V4])
+@pytest.mark.parametrize("n_seq,rows,new,window", [(1, 293, 7, 0), (2, 60, 5, 0), (3, 300, 1, 64), (4, 2000, 16, 0), (4, 2000, 16, 100)])
+def test_what_masked_rows_hold(torch, preset, e4m3, bad, n_seq, rows, new, window):
+    """Rows that a token does not see hold NaN, infinities or huge values, in the latent or the rope dims: the bits of its
+    output are those with ordinary rows in their place.  (Rows of later tokens; rows in front of the window.)"""
+    rng = np.random.default_rng(17)
+    n = rows + new
+    with make(preset, e4m3=e4m3, n_pages=40 * n_seq) as ctx:
+        row = ctx.dims["row"]
+        w = {k: np.zeros(sh, np.uint16) for k, sh in mla.weight_shapes(ctx.cfg).items()}
+        w["attn_sinks"] = np.zeros(64, np.float32)
+        ctx.set_layer_weights(0, w)
+        x = rng.standard_normal((n_seq, n, row)).astype(np.float32)
+        q = dev(torch, bits(rng.standard_normal((n_seq * new * 64, row)).astype(np.float32)))
+        o = dev(torch, np.zeros((n_seq * new * 64, 512), np.uint16))
+        seqs = [ctx.seq_alloc() for _ in range(n_seq)]
+        first = new // 2  # tokens from here on see bad rows of later tokens
+        outs = []
+        for spoiled in (False, True):
+            y = x.copy()
+            if spoiled:
+                for b in range(n_seq):
+                    if new > 1:
+                        y[b, rows + first, 5 + b] = bad
+                        y[b, n - 1, 400] = -bad
+                        y[b, n - 2, row - 3] = bad
+                    if window:
+                        y[b, rows - window - 8, 77] = bad
+                        y[b, rows - window - 20] = bad
+                        y[b, rows - window - 30, row - 1] = bad
+            for s, r in zip(seqs, y):
+                ctx.cache_write(0, s, 0, bits(r))
+            ctx.plan([(s, rows, new, -1, 1, window) for s in seqs], causal=True)
+            ctx.attention_device(0, q.data_ptr(), o.data_ptr())
+            ctx.sync()
+            outs.append(host(o).reshape(n_seq, new, 64, 512))
+        sees_none = first if new > 1 else 1
+        assert np.isfinite(f32(outs[0])).all()
+        assert np.array_equal(outs[0][:, :sees_none], outs[1][:, :sees_none])
+        if new > 1 and not math.isfinite(bad) and not (e4m3 and math.isinf(bad)):
+            assert np.isnan(f32(outs[1][:, first:])).any((2, 3)).all()  # who sees the row has it
+
+
 def test_attention_without_rows(torch):
     """Tokens that see nothing get zeros, also beside tokens that see something."""
     with make() as ctx:

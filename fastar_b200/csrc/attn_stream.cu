@@ -778,34 +778,37 @@ k_attn_stream(const __grid_constant__ CUtensorMap tmKV, const __grid_constant__ 
         if (!WHOLE) tc::mbar_arrive(&mi->s_free[b1]);
         float mx = -INFINITY;
         const int tile0 = (sg.kv_begin & ~(TILE - 1)) - sg.kv_begin + t * TILE;
-        // Tiles that the token sees whole need no masks.  With / without a path of their own, us, bf16: 64 users over
-        // 1024-8192 rows 71.0 / 72.4, 32 x 16 new tokens over 16384 rows 1197 / 1212, a prompt of 2000 rows 895 / 901;
-        // E4M3, 64 users 79.6 / 78.6 (two registers more where there is none left).
-        if (!E8 && tile0 >= 0 && (unsigned)(tile0 + TILE) <= span) {
+        // Blocks of query tokens (WHOLE): tiles that the token sees whole need no masks.  With / without a path of their
+        // own, us, bf16: 32 x 16 new tokens over 16384 rows 1211 / 1230, a prompt of 2000 rows 895 / 909.  One token of many
+        // users: 71.4 / 71.2; E4M3, 64 users: 79.6 / 78.6 (two registers more where there is none left).
+        if (WHOLE && !E8 && tile0 >= 0 && (unsigned)(tile0 + TILE) <= span) {
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            sc[j] = (sc[j] + sc2[j]) * p.scale_log2;
+            sc[j] *= p.scale_log2;
             mx = fmaxf(mx, sc[j]);
           }
         } else {
-          // Rows of the tile that the token does not see get a probability of 0, and 0 times an infinity or a NaN that one
-          // holds (a later token's, one's before the window) would still reach the output.  Such a row's scores are not
-          // finite, for every head; the thread of a head then clears one of the row's 64 16-byte units of latent
-          // values.  (The tile's QK MMAs have retired, its SV MMAs wait for p_full.)  E8: they came in as zeros.
-          uint32_t clear = 0;
+          float bad0 = 0.0f, bad1 = 0.0f;  // NaN when a score of the tile is not finite
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             const float x = (sc[j] + sc2[j]) * p.scale_log2;
-            const bool seen = (unsigned)(rel0 + j) < span;
-            if (!E8 && !seen && !(fabsf(x) < INFINITY)) clear |= 1u << j;
-            sc[j] = seen ? x : -INFINITY;
+            if (!E8) (j & 1 ? bad1 : bad0) = fmaf(x, 0.0f, j & 1 ? bad1 : bad0);
+            sc[j] = (unsigned)(rel0 + j) < span ? x : -INFINITY;
             mx = fmaxf(mx, sc[j]);
           }
+          // Rows of the tile that the token does not see get a probability of 0, and 0 times an infinity or a NaN that one
+          // holds (a later token's, one's before the window) would still reach the output.  Such a row's scores are not
+          // finite, for every head; the thread of a head then clears one of the 64 16-byte units of latent values of
+          // the unseen rows.  (The tile's QK MMAs have retired, its SV MMAs wait for p_full.)  E8: they came in as
+          // zeros.  What the search costs, us: a layer call for one token over 4096 rows (a tile per block) 62.1 / 61.7.
+          if (!E8 && bad0 + bad1 != 0.0f) {
 #pragma unroll 1
-          for (; clear; clear &= clear - 1) {
-            const int tok = half * 32 + sub * 16 + __ffs(clear) - 1;
-            *reinterpret_cast<uint4*>(s_ring + ((g % F) * NCH + (row >> 3)) * CHUNK + tok * 128 + (((row & 7) ^ (tok & 7)) * 16)) =
-                make_uint4(0, 0, 0, 0);
+            for (int j = 0; j < 16; ++j) {
+              const int tok = half * 32 + sub * 16 + j;
+              if ((unsigned)(rel0 + j) >= span)
+                *reinterpret_cast<uint4*>(s_ring + ((g % F) * NCH + (row >> 3)) * CHUNK + tok * 128 + (((row & 7) ^ (tok & 7)) * 16)) =
+                    make_uint4(0, 0, 0, 0);
+            }
           }
         }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
